@@ -163,7 +163,8 @@ def _blocks(x):
 
 def _quantize(x):
     """(codes, scales) of a Float32 matrix: two e2m1 values to a byte, the one of the lower k in the low half, and one
-    e8m0 byte for 32 values along k: floor(log2(largest magnitude)) - 2, or 255 where one is not finite."""
+    e8m0 byte for 32 values along k: floor(log2(largest magnitude)) - 2, or 255 where one is not finite.  Scales lie in
+    panels of eight blocks (256 values of k), the rows of a panel one after the other, eight bytes each."""
     v = _blocks(x)
     top = v.abs().amax(-1)
     exponent = torch.where(top > 0, torch.frexp(top)[1] - 3, -127).clamp(-127, 127)
@@ -173,12 +174,26 @@ def _quantize(x):
     code = code + 8 * torch.signbit(scaled).to(torch.uint8)
     code = code.view(v.shape[0], -1)
     scales = torch.where(torch.isfinite(top), exponent + 127, 255).to(torch.uint8)
-    return (code[:, 0::2] + 16 * code[:, 1::2]).contiguous(), scales
+    rows, blocks = scales.shape
+    panels = torch.zeros(_panels(rows, x.shape[1]), dtype=torch.uint8, device=x.device)
+    padded = torch.zeros((panels.shape[1], panels.shape[0] * 8), dtype=torch.uint8, device=x.device)
+    padded[:rows, :blocks] = scales
+    panels.copy_(padded.view(panels.shape[1], -1, 8).transpose(0, 1))
+    return (code[:, 0::2] + 16 * code[:, 1::2]).contiguous(), panels
 
 
-def _dequantize(codes, scales, k, dtype=torch.float32):
-    table = torch.tensor(E2M1, dtype=dtype, device=codes.device)
-    values = torch.stack((table[(codes & 15).int()], table[(codes >> 4).int()]), -1).view(codes.shape[0], scales.shape[1], 32)
+def _panels(rows, k):
+    return -(-k // 256), rows + rows % 2, 8
+
+
+def _row_scales(codes, panels):
+    """One row of scales for each row of codes."""
+    return panels.transpose(0, 1).reshape(panels.shape[1], -1)[:codes.shape[0], :codes.shape[1] // 16]
+
+
+def _dequantize(codes, panels, k, dtype=torch.float32):
+    table, scales = torch.tensor(E2M1, dtype=dtype, device=codes.device), _row_scales(codes, panels)
+    values = torch.stack((table[(codes & 15).int()], table[(codes >> 4).int()]), -1).view(codes.shape[0], -1, 32)
     factor = torch.where(scales == 255, math.nan, torch.ldexp(torch.ones((), dtype=dtype, device=codes.device), scales.int() - 127))
     return (values * factor[..., None]).view(codes.shape[0], -1)[:, :k]
 
@@ -229,7 +244,7 @@ def prepare(case, seed):
         # rows of different size, a few of zeros
         x = torch.empty((rows, k), device="cuda").normal_(0.0, 1.0, generator=gen) * torch.exp(torch.randn((rows, 1), device="cuda", generator=gen))
         x[torch.rand(rows, device="cuda", generator=gen) < 0.01] = 0.0
-        state.update(x=x.to(_TORCH[case["type"]]), codes=empty((rows, 16 * blocks), torch.uint8), scales=empty((rows, blocks), torch.uint8), back=empty((rows, k), "bf16"))
+        state.update(x=x.to(_TORCH[case["type"]]), codes=empty((rows, 16 * blocks), torch.uint8), scales=empty(_panels(rows, k), torch.uint8), back=empty((rows, k), "bf16"))
     elif op == "mxfp4":
         state.update(a=_mxfp4_codes(gen, case["m"], case["k"], 1.0), b=_mxfp4_codes(gen, case["n"], case["k"], 0.02), y=empty((case["m"], case["n"]), case["out"]))
     else:
@@ -421,8 +436,9 @@ def exact(case, seed):
     return torch.matmul(_value64(*s["a"], case["k"]), _value64(*s["b"], case["k"]).transpose(0, 1).contiguous())
 
 
-def _value64(codes, scales, k):
+def _value64(codes, panels, k):
     """What codes and scales stand for, from the fields of e2m1: sign, two bits of exponent, one of mantissa."""
+    scales = _row_scales(codes, panels)
     nibble = torch.stack((codes % 16, codes // 16), -1).view(codes.shape[0], -1).double()
     sign = torch.where(nibble >= 8, -1.0, 1.0).double()
     nibble = nibble % 8
