@@ -14,6 +14,9 @@ from .execution import (HostKernel, Module, Stream, cuda, cufunction, cudaconver
                         warpsize, nextwarp, prevwarp)
 from . import wmma as WMMA
 from . import gemm as GEMM
+from . import experts as EXPERTS
+from . import mxfp4 as MXFP4
+from .experts import BFloat16
 from . import reflection
 from . import launch_overhead
 

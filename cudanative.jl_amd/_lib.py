@@ -11,7 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MIWMMA_LIB") or os.path.join(HERE, "libmiwmma.so")
 
 ROW_MAJOR, COL_MAJOR = 0, 1
-F16, F32 = 0, 1
+F16, F32, BF16 = 0, 1, 2
+EPILOGUE_NONE, EPILOGUE_GATED_SILU = 0, 1
 MATRIX_A, MATRIX_B, ACCUMULATOR = 0, 1, 2
 AS_GENERIC, AS_GLOBAL, AS_SHARED = 0, 1, 3
 OP_MUL, OP_ADD = 0, 1
@@ -155,6 +156,18 @@ SIGNATURES = {
     "miw_mfma_power_probe": (_i, [_i, _i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double), _vp]),
     "miw_mfma_peak_probe": (_i, [_i, ctypes.POINTER(ctypes.c_double), _vp]),
     "miw_copy_probe": (_i, [_vp, _vp, _sz, _vp]),
+    "miw_route_workspace": (_i, [_i64, _i, _i, ctypes.POINTER(_sz)]),
+    "miw_route": (_i, [_i, _i64, _i, _i, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "miw_route_grad": (_i, [_i, _i64, _i, _i, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_grouped_gemm": (_i, [_i, _i, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_grouped_wgrad": (_i, [_i, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_combine": (_i, [_i, _i64, _i, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "miw_combine_grad": (_i, [_i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_mxfp4_quantize": (_i, [_i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "miw_mxfp4_dequantize": (_i, [_i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "miw_mxfp4_gemm": (_i, [_i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_mxfp4_grouped_gemm": (_i, [_i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                    _vp, _vp]),
     "miw_kernel_count": (_i, []),
     "miw_kernel_name": (_i, [_i, ctypes.c_char_p, _sz]),
     "miw_kernel_lookup": (_i, [ctypes.c_char_p, _vpp]),

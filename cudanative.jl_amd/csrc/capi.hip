@@ -3,6 +3,7 @@
 // Nothing here falls back to the CPU: without a usable HIP device every entry
 // that needs one returns the HIP error.
 #include "../../include/miwmma.h"
+#include "api_common.hpp"
 #include "kernels.hpp"
 
 #include <hip/hip_runtime.h>
@@ -590,6 +591,22 @@ int launch_parts(const miw_gemm_desc *d, const std::vector<gemm_part> &parts, bo
 }
 
 }  // namespace
+
+namespace miw {
+
+int api_fail(int code, const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int api_hip_fail(hipError_t e, const char *what) { return hip_fail(e, what); }
+bool api_initialized() { return g_initialized.load(std::memory_order_acquire); }
+int api_cu_count() { return cu_count(); }
+
+}  // namespace miw
 
 extern "C" {
 

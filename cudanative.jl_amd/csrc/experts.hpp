@@ -1,0 +1,83 @@
+// Declarations shared by the experts' kernels, the 4-bit conversions and their C ABI layer.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace miw {
+
+// Element types, numbered as MIW_F16, MIW_F32, MIW_BF16.
+enum { TYPE_F16 = 0, TYPE_F32 = 1, TYPE_BF16 = 2 };
+
+// --- route.hip
+struct route_params {
+    const void *logits;
+    int *chosen;
+    float *gates;
+    int *offsets, *rows, *place;
+    int *counts;  // workspace: choices of each expert in each chunk of tokens
+    int tokens, experts, top, over_all;
+    long ld;
+    int chunks, chunk;  // chunks of `chunk` tokens
+};
+// Chunks that the tokens are cut into; 1: one workgroup does everything and there is no workspace.
+int route_chunks(long tokens, int top);
+hipError_t launch_route(route_params p, int dtype, hipStream_t s);
+struct route_grad_params {
+    const void *logits;
+    const int *chosen;
+    const float *gates, *dgates;
+    void *dlogits;
+    int tokens, experts, top, over_all;
+    long ld, ldd;
+};
+hipError_t launch_route_grad(const route_grad_params &p, int dtype, hipStream_t s);
+
+// --- combine.hip
+struct combine_params {
+    const void *H, *dY;
+    const float *gates;  // or null: 1
+    const int *place;
+    void *out;      // Y, or dH
+    float *dgates;  // or null
+    int tokens, top, rows;
+    long n, ldh, ldy, lddh;
+    int vector;  // 16-byte accesses: pointers, pitches and n allow them
+};
+hipError_t launch_combine(const combine_params &p, int dtype, hipStream_t s);
+hipError_t launch_combine_grad(const combine_params &p, int dtype, hipStream_t s);
+
+// --- mxfp4_convert.hip
+struct mxfp4_convert_params {
+    const void *in;
+    void *out;
+    uint8_t *codes, *scales;
+    long rows, k, ld, ldq, lds;
+    int vector;  // 16-byte accesses to the matrix
+};
+hipError_t launch_mxfp4_quantize(const mxfp4_convert_params &p, int dtype, hipStream_t s);
+hipError_t launch_mxfp4_dequantize(const mxfp4_convert_params &p, int dtype, hipStream_t s);
+
+// --- grouped_*.hip
+// D[j][i] = sum over k of X_g[i][k] * Y[j][k]: i runs along D's rows (contiguous), j over rows of D.
+//   Rows are ragged (miw_grouped_gemm): X is the group's weights, Y the rows of A that gather names.
+//   The sum is ragged (miw_grouped_wgrad): k runs over a group's rows, X is B (gathered), Y is A, D the group's own.
+struct grouped_params {
+    const char *X, *Y;
+    const uint8_t *xs, *ys;  // scales of 4-bit operands
+    const int *offsets, *gather;
+    void *D;
+    int groups, rows, source_rows;  // source_rows: of the operand that gather names
+    int I, J, K;                    // J: only where the sum is ragged; K: only where the rows are
+    long ldx, ldy, ldd;             // X, Y: bytes; D: elements
+    long sx, sd, sxs;               // from group to group: X and scales in bytes, D in elements
+    long lxs, lys;                  // rows of a panel of scales
+    int x_k_major;                  // k contiguous in X
+    int gated, accumulate;
+    int vector;   // 16-byte accesses to the operands
+    int d_vector; // aligned stores of four elements
+};
+hipError_t launch_grouped_plain(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
+hipError_t launch_grouped_mxfp4_plain(const grouped_params &p, int d_type, hipStream_t s);
+
+}  // namespace miw

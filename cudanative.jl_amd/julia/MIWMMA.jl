@@ -30,7 +30,9 @@ module MIWMMA
 
 export DeviceBuffer, DevicePtr, AS, WMMA, @hip, gemm!, gemm_splitk!, gemm_splitk_static!, synchronize, MIWError,
        HostKernel, hipfunction, CodeObject, kernel, registers, memory, maxthreads, launch_configuration,
-       Stream, device_info, warpsize, nextwarp, prevwarp, mem_info
+       Stream, device_info, warpsize, nextwarp, prevwarp, mem_info,
+       route!, route_grad!, grouped_gemm!, grouped_wgrad!, combine!, combine_grad!,
+       mxfp4_quantize!, mxfp4_dequantize!, mxfp4_gemm!, mxfp4_grouped_gemm!
 
 const libmiwmma = get(ENV, "MIWMMA_LIB", joinpath(@__DIR__, "..", "libmiwmma.so"))
 
@@ -815,6 +817,125 @@ end
 
 function copy_probe(dst::DeviceBuffer, src::DeviceBuffer, bytes::Integer; stream=C_NULL)
     check(ccall((:miw_copy_probe, libmiwmma), Cint, (Ptr{Cvoid}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}), dst.ptr, src.ptr, bytes, stream_handle(stream)))
+end
+
+# ---------------------------------------------------------------------------- experts -----
+# A layer of experts and microscaled 4-bit matrices (include/miwmma.h says what each does).  Matrices are row-major in
+# memory: the last index of a matrix is the first of the DeviceBuffer that holds it.  Julia has no 16-bit brain float of
+# its own: `dtype` (and `d_type`) name the elements as :f16, :bf16 or :f32, whatever the buffers' element type.
+
+const ELEMENT_CODES = Dict(:f16 => Cint(0), :f32 => Cint(1), :bf16 => Cint(2))
+address(x) = x === nothing ? C_NULL : x.ptr
+epilogue_code(e::Symbol) = e === :none ? Cint(0) : e === :gated_silu ? Cint(1) : throw(ArgumentError("epilogue is :none or :gated_silu"))
+
+"Bytes of workspace that route! needs (0: none)."
+function route_workspace(tokens::Integer, experts::Integer, top::Integer)
+    n = Ref{Csize_t}(0)
+    check(ccall((:miw_route_workspace, libmiwmma), Cint, (Int64, Cint, Cint, Ptr{Csize_t}), tokens, experts, top, n))
+    return Int(n[])
+end
+
+"The `top` largest logits of each token, their softmax, and the order of the rows by expert."
+function route!(chosen, gates, offsets, rows, place, logits; tokens::Integer, experts::Integer, top::Integer, dtype::Symbol=:f32,
+                ld::Integer=0, over_all::Bool=false, workspace=nothing, workspace_bytes::Integer=0, stream=C_NULL)
+    GC.@preserve chosen gates offsets rows place logits workspace check(ccall((:miw_route, libmiwmma), Cint,
+        (Cint, Int64, Cint, Cint, Int64, Cint, Ptr{Cvoid}, Ptr{Cint}, Ptr{Cfloat}, Ptr{Cint}, Ptr{Cint}, Ptr{Cint}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], tokens, experts, top, ld, over_all ? 1 : 0, address(logits), address(chosen), address(gates), address(offsets),
+        address(rows), address(place), address(workspace), workspace_bytes, stream_handle(stream)))
+    return chosen
+end
+
+function route_grad!(dlogits, logits, chosen, gates, dgates; tokens::Integer, experts::Integer, top::Integer, dtype::Symbol=:f32,
+                     ld::Integer=0, ldd::Integer=0, over_all::Bool=false, stream=C_NULL)
+    GC.@preserve dlogits logits chosen gates dgates check(ccall((:miw_route_grad, libmiwmma), Cint,
+        (Cint, Int64, Cint, Cint, Int64, Int64, Cint, Ptr{Cvoid}, Ptr{Cint}, Ptr{Cfloat}, Ptr{Cfloat}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], tokens, experts, top, ld, ldd, over_all ? 1 : 0, address(logits), address(chosen), address(gates), address(dgates),
+        address(dlogits), stream_handle(stream)))
+    return dlogits
+end
+
+"D[r] = A[gather[r]] * W_g on the rows of each group; `w_layout` 1 (column-major): k contiguous in W."
+function grouped_gemm!(D, A, W, offsets; rows::Integer, groups::Integer, n::Integer, k::Integer, dtype::Symbol=:f16, d_type::Symbol=dtype,
+                       w_layout::Integer=1, epilogue::Symbol=:none, gather=nothing, a_rows::Integer=0, lda::Integer=0, ldw::Integer=0,
+                       stride_w::Integer=0, ldd::Integer=0, stream=C_NULL)
+    GC.@preserve D A W offsets gather check(ccall((:miw_grouped_gemm, libmiwmma), Cint,
+        (Cint, Cint, Cint, Cint, Int64, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cint},
+         Ptr{Cint}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], ELEMENT_CODES[d_type], w_layout, epilogue_code(epilogue), rows, groups, n, k, lda, ldw, stride_w, ldd, a_rows,
+        address(A), address(W), address(D), address(offsets), address(gather), stream_handle(stream)))
+    return D
+end
+
+"D_g = sum over the rows of group g of A[r]^T * B[gather[r]]."
+function grouped_wgrad!(D, A, B, offsets; rows::Integer, groups::Integer, m::Integer, n::Integer, dtype::Symbol=:f16, d_type::Symbol=:f32,
+                        accumulate::Bool=false, gather=nothing, b_rows::Integer=0, lda::Integer=0, ldb::Integer=0, ldd::Integer=0,
+                        stride_d::Integer=0, stream=C_NULL)
+    GC.@preserve D A B offsets gather check(ccall((:miw_grouped_wgrad, libmiwmma), Cint,
+        (Cint, Cint, Cint, Int64, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cint},
+         Ptr{Cint}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], ELEMENT_CODES[d_type], accumulate ? 1 : 0, rows, groups, m, n, lda, ldb, ldd, stride_d, b_rows,
+        address(A), address(B), address(D), address(offsets), address(gather), stream_handle(stream)))
+    return D
+end
+
+"Y[t] = sum over j of gates[t, j] * H[place[t, j]]."
+function combine!(Y, H, place; tokens::Integer, top::Integer, n::Integer, rows::Integer, gates=nothing, dtype::Symbol=:f16, ldh::Integer=0,
+                  ldy::Integer=0, stream=C_NULL)
+    GC.@preserve Y H place gates check(ccall((:miw_combine, libmiwmma), Cint,
+        (Cint, Int64, Cint, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cint}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], tokens, top, n, rows, ldh, ldy, address(H), address(gates), address(place), address(Y), stream_handle(stream)))
+    return Y
+end
+
+function combine_grad!(dH, dgates, dY, H, place; tokens::Integer, top::Integer, n::Integer, rows::Integer, gates=nothing,
+                       dtype::Symbol=:f16, ldy::Integer=0, ldh::Integer=0, lddh::Integer=0, stream=C_NULL)
+    GC.@preserve dH dgates dY H place gates check(ccall((:miw_combine_grad, libmiwmma), Cint,
+        (Cint, Int64, Cint, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cfloat}, Ptr{Cint}, Ptr{Cvoid}, Ptr{Cfloat},
+         Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], tokens, top, n, rows, ldy, ldh, lddh, address(dY), address(H), address(gates), address(place), address(dH),
+        address(dgates), stream_handle(stream)))
+    return dH
+end
+
+"X (rows x k) into 4-bit codes and scales."
+function mxfp4_quantize!(codes, scales, X; rows::Integer, k::Integer, dtype::Symbol=:f16, ld::Integer=0, ldq::Integer=0, lds::Integer=0,
+                         stream=C_NULL)
+    GC.@preserve codes scales X check(ccall((:miw_mxfp4_quantize, libmiwmma), Cint,
+        (Cint, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], rows, k, ld, ldq, lds, address(X), address(codes), address(scales), stream_handle(stream)))
+    return codes
+end
+
+function mxfp4_dequantize!(X, codes, scales; rows::Integer, k::Integer, dtype::Symbol=:f32, ldq::Integer=0, lds::Integer=0, ld::Integer=0,
+                           stream=C_NULL)
+    GC.@preserve codes scales X check(ccall((:miw_mxfp4_dequantize, libmiwmma), Cint,
+        (Cint, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], rows, k, ldq, lds, ld, address(codes), address(scales), address(X), stream_handle(stream)))
+    return X
+end
+
+"D (m x n) = A * B^T with both in 4 bits."
+function mxfp4_gemm!(D, A, A_scales, B, B_scales; m::Integer, n::Integer, k::Integer, d_type::Symbol=:f16, epilogue::Symbol=:none,
+                     lda::Integer=0, lds_a::Integer=0, ldb::Integer=0, lds_b::Integer=0, ldd::Integer=0, stream=C_NULL)
+    GC.@preserve D A A_scales B B_scales check(ccall((:miw_mxfp4_gemm, libmiwmma), Cint,
+        (Cint, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+         Ptr{Cvoid}),
+        ELEMENT_CODES[d_type], epilogue_code(epilogue), m, n, k, lda, lds_a, ldb, lds_b, ldd, address(A), address(A_scales), address(B),
+        address(B_scales), address(D), stream_handle(stream)))
+    return D
+end
+
+"grouped_gemm! with A and the groups' n x k matrices in 4 bits."
+function mxfp4_grouped_gemm!(D, A, A_scales, W, W_scales, offsets; rows::Integer, groups::Integer, n::Integer, k::Integer,
+                             d_type::Symbol=:f16, epilogue::Symbol=:none, gather=nothing, a_rows::Integer=0, lda::Integer=0,
+                             lds_a::Integer=0, ldw::Integer=0, lds_w::Integer=0, stride_w::Integer=0, stride_ws::Integer=0, ldd::Integer=0,
+                             stream=C_NULL)
+    GC.@preserve D A A_scales W W_scales offsets gather check(ccall((:miw_mxfp4_grouped_gemm, libmiwmma), Cint,
+        (Cint, Cint, Int64, Cint, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+         Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cint}, Ptr{Cint}, Ptr{Cvoid}),
+        ELEMENT_CODES[d_type], epilogue_code(epilogue), rows, groups, n, k, lda, lds_a, ldw, lds_w, stride_w, stride_ws, ldd, a_rows,
+        address(A), address(A_scales), address(W), address(W_scales), address(D), address(offsets), address(gather), stream_handle(stream)))
+    return D
 end
 
 end # module MIWMMA

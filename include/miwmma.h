@@ -38,6 +38,8 @@ extern "C" {
 enum { MIW_ROW_MAJOR = 0, MIW_COL_MAJOR = 1 };
 /* Element types WMMA accepts (src/device/cuda/wmma.jl:11-15). */
 enum { MIW_F16 = 0, MIW_F32 = 1 };
+/* A third element type, of the experts' operators and the 4-bit conversions only (no counterpart in the reference). */
+enum { MIW_BF16 = 2 };
 /* FragmentUse: MatrixA / MatrixB / Accumulator (src/device/cuda/wmma.jl:343-346). */
 enum { MIW_MATRIX_A = 0, MIW_MATRIX_B = 1, MIW_ACCUMULATOR = 2 };
 /* Address spaces, numbered as AS.Generic/Global/Shared (src/device/pointer.jl:11-27).
@@ -336,6 +338,90 @@ int miw_launch_overhead_probe(int iters, int threads, float *cpu_us, float *gpu_
 
 /* Plain device copy kernel (16 B per lane), used to calibrate HBM counters. */
 int miw_copy_probe(void *dst, const void *src, size_t bytes, void *stream);
+
+/* ---------------------------------------------------------------- experts -- */
+/* A layer of experts: every token goes to a few of many matrices.  No counterpart in the reference; the products are the
+   chain of mma calls of docs/src/device/wmma.md:51-52 on rows that lie sorted by expert.
+     miw_route         which experts a token goes to, with which weights, and where its rows lie in the sorted order
+     miw_grouped_gemm  the rows of each expert times its matrix (forward pass, and gradient to the rows)
+     miw_grouped_wgrad the gradient to each expert's matrix
+     miw_combine       a token's answers joined by its weights
+   Nothing here waits for the device: how many rows an expert has is only known there, and stays there (`offsets`).
+   Matrices are row-major; a leading dimension or stride of 0 means "dense".  Element types: MIW_F16, MIW_BF16 and, where
+   said, MIW_F32.  Results share no memory with operands. */
+
+/* route.  logits: tokens x experts (F16, BF16 or F32), row pitch ld.  For every token the `top` largest logits are chosen, in
+   falling order, equal ones by rising expert number.  A logit of -inf or NaN is never chosen;
+   where fewer than `top` are left the remaining choices are -1, with weight 0.  +inf counts as the largest finite Float32.
+     chosen [tokens x top]   expert of each choice, or -1
+     gates  [tokens x top]   softmax over the chosen logits, or with over_all over all of the token's
+     offsets [experts + 1]   sorted positions offsets[e] .. offsets[e + 1] - 1 belong to expert e
+     rows   [tokens * top]   token at each sorted position (by expert, then by token); -1 from offsets[experts] on
+     place  [tokens x top]   sorted position of each choice, or -1
+   At most 1024 experts, top of at most 16 and of `experts`, tokens * top at most 2^30.  The workspace (miw_route_workspace bytes, 16-byte
+   aligned; 0 bytes: it may be null) needs no clearing.  The same bits every time. */
+int miw_route_workspace(int64_t tokens, int experts, int top, size_t *bytes);
+int miw_route(int dtype, int64_t tokens, int experts, int top, int64_t ld, int over_all, const void *logits, int *chosen,
+              float *gates, int *offsets, int *rows, int *place, void *workspace, size_t workspace_bytes, void *stream);
+/* The gradient to the logits (tokens x experts, row pitch ldd, of the logits' type), from the gradient to the gates; every element is written. */
+int miw_route_grad(int dtype, int64_t tokens, int experts, int top, int64_t ld, int64_t ldd, int over_all, const void *logits,
+                   const int *chosen, const float *gates, const float *dgates, void *dlogits, void *stream);
+
+/* What a product does with its sums before it rounds and stores them.  GATED_SILU: columns 2c and 2c + 1 are a gate and a
+   value, and column c of D (n / 2 wide) is gate / (1 + exp(-gate)) * value, in Float32; n is even. */
+enum { MIW_EPILOGUE_NONE = 0, MIW_EPILOGUE_GATED_SILU = 1 };
+
+/* D[r] = A[gather[r]] * W_g for the sorted positions r of each group g, offsets[g] <= r < offsets[g + 1]; gather null:
+   A[r].  W_g is k x n: n x k in memory with MIW_COL_MAJOR (k contiguous, as a layer keeps its weights), k x n with
+   MIW_ROW_MAJOR (the same weights in the gradient to the rows: dX = dY * W).  rows: sorted positions there are at most (D's
+   rows); those outside the groups are not touched.  a_rows: rows of A, those that gather names (0: as many as `rows`).
+   offsets outside 0 .. rows and gather outside 0 .. a_rows - 1 are taken as the nearest value inside.  d_type: dtype or MIW_F32; sums are Float32.
+   Any sizes; 16-byte aligned operands with k, n and pitches in multiples of 8 elements run on the faster kernels. */
+int miw_grouped_gemm(int dtype, int d_type, int w_layout, int epilogue, int64_t rows, int groups, int64_t n, int64_t k,
+                     int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldd, int64_t a_rows, const void *A, const void *W,
+                     void *D, const int *offsets, const int *gather, void *stream);
+/* D_g (m x n) = sum over the rows r of group g of A[r]^T * B[gather[r]]: with A = dY and B = X the gradient to weights that lie
+   m x n.  A group without rows gets zeros.  accumulate: added to what D holds (an empty group's is not touched). */
+int miw_grouped_wgrad(int dtype, int d_type, int accumulate, int64_t rows, int groups, int64_t m, int64_t n, int64_t lda,
+                      int64_t ldb, int64_t ldd, int64_t stride_d, int64_t b_rows, const void *A, const void *B, void *D,
+                      const int *offsets, const int *gather, void *stream);
+
+/* Y[t] = sum over j of gates[t][j] * H[place[t][j]], in the order of j (gates null: 1, which joins gradients to rows that
+   were gathered).  A place outside 0 .. rows - 1 adds nothing.  H: rows x n, Y: tokens x n. */
+int miw_combine(int dtype, int64_t tokens, int top, int64_t n, int64_t rows, int64_t ldh, int64_t ldy, const void *H,
+                const float *gates, const int *place, void *Y, void *stream);
+/* dH[place[t][j]] = gates[t][j] * dY[t] (rows that no place names are not touched), dgates[t][j] = dY[t] . H[place[t][j]]
+   (0 without a place).  dgates null: H is not read and may be null. */
+int miw_combine_grad(int dtype, int64_t tokens, int top, int64_t n, int64_t rows, int64_t ldy, int64_t ldh, int64_t lddh,
+                     const void *dY, const void *H, const float *gates, const int *place, void *dH, float *dgates, void *stream);
+
+/* ------------------------------------------------- microscaled 4-bit floats -- */
+/* A matrix of rows x k values of e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with one e8m0 scale for 32 along k.
+     codes   two values to a byte, the one of the lower k in the low half; rows of ldq bytes, a multiple of 16 and at least
+             16 * ceil(k / 32), on 16-byte addresses.  What a last block has beyond k is written as zeros.
+     scales  in panels of eight blocks: byte ((p * lds + r) * 8 + b) is the scale of row r's block 8 p + b, for
+             ceil(k / 256) panels of lds rows (an even number of at least `rows`), on 16-byte addresses.
+   Pitches of 0: dense (16 * ceil(k / 32) bytes; rows rounded up to an even number). */
+
+/* A block's scale is 2^(floor(log2(its largest magnitude)) - 2), kept in -127 .. 127; its values are divided by that,
+   rounded to the nearest (ties to the even code) and kept within 6.  A block of zeros has scale 0 (2^-127); one that holds an
+   infinity or a NaN gets scale 255, which stands for NaN.  dtype: F16, BF16 or F32.  Blocks that the last panel has beyond
+   k get scale 0. */
+int miw_mxfp4_quantize(int dtype, int64_t rows, int64_t k, int64_t ld, int64_t ldq, int64_t lds, const void *X, void *codes,
+                       void *scales, void *stream);
+/* What codes and scales stand for, as F16, BF16 (always exact) or F32. */
+int miw_mxfp4_dequantize(int dtype, int64_t rows, int64_t k, int64_t ldq, int64_t lds, int64_t ld, const void *codes,
+                         const void *scales, void *X, void *stream);
+/* D (m x n, row-major) = A * B^T, A m x k and B n x k in 4 bits; Float32 sums, D F16, BF16 or F32. */
+int miw_mxfp4_gemm(int d_type, int epilogue, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t lds_a, int64_t ldb,
+                   int64_t lds_b, int64_t ldd, const void *A, const void *A_scales, const void *B, const void *B_scales, void *D,
+                   void *stream);
+/* miw_grouped_gemm with A and W in 4 bits, W_g as n x k.  stride_w, stride_ws: bytes from one group's codes and scales to the next
+   (multiples of 16; 0: dense). */
+int miw_mxfp4_grouped_gemm(int d_type, int epilogue, int64_t rows, int groups, int64_t n, int64_t k, int64_t lda, int64_t lds_a,
+                           int64_t ldw, int64_t lds_w, int64_t stride_w, int64_t stride_ws, int64_t ldd, int64_t a_rows,
+                           const void *A, const void *A_scales, const void *W, const void *W_scales, void *D, const int *offsets,
+                           const int *gather, void *stream);
 
 /* ----------------------------------------------------------- generic launch */
 /* @cuda threads= blocks= shmem= stream= f(args...) (src/execution.jl:45-114)
