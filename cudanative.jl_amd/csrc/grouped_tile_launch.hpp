@@ -1,0 +1,49 @@
+// Instances of k_grouped_tile for one element type and their launch.
+#pragma once
+#include "grouped_tile.hpp"
+
+#include <type_traits>
+
+namespace miw {
+
+template <class OP, int BI, int BJ, int WI, int WJ, int NSLOT, int FORM, class DT>
+static hipError_t launch_tile_instance(const grouped_params &p, hipStream_t s)
+{
+    constexpr int lds = grouped_lds_bytes(BI, BJ, NSLOT, OP::scaled, FORM);
+    const void *fn = (const void *)k_grouped_tile<OP, BI, BJ, WI, WJ, NSLOT, FORM, DT>;
+    static const hipError_t allowed = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (allowed != hipSuccess) return allowed;
+    const long blocks = FORM == RAGGED_SUM ? (long)p.groups * ((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ) : grouped_blocks(p, BI, BJ, 512);
+    if (blocks <= 0 || blocks >= 1l << 23) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((k_grouped_tile<OP, BI, BJ, WI, WJ, NSLOT, FORM, DT>), dim3((unsigned)blocks), dim3(512), lds, s, p);
+    return hipGetLastError();
+}
+
+template <class OP, int FORM, class DT>
+static hipError_t launch_tile_size(const grouped_params &p, grouped_tile_size t, hipStream_t s)
+{
+    switch (t) {
+    case TILE_256x128: return launch_tile_instance<OP, 256, 128, 4, 2, 3, FORM, DT>(p, s);
+    case TILE_128x128: return launch_tile_instance<OP, 128, 128, 4, 2, 4, FORM, DT>(p, s);
+    default: return launch_tile_instance<OP, 128, 64, 4, 2, 6, FORM, DT>(p, s);
+    }
+}
+
+// T: the 16-bit type of results that are not Float32.
+template <class OP, class T>
+static hipError_t launch_tile(const grouped_params &p, grouped_tile_size t, int d_type, bool ragged_sum, hipStream_t s)
+{
+    auto go = [&](auto type) {
+        using DT = decltype(type);
+        if constexpr (OP::scaled) {
+            return launch_tile_size<OP, ROWS_X_K, DT>(p, t, s);
+        } else {
+            if (ragged_sum) return launch_tile_size<OP, RAGGED_SUM, DT>(p, t, s);
+            return p.x_k_major ? launch_tile_size<OP, ROWS_X_K, DT>(p, t, s) : launch_tile_size<OP, ROWS_X_I, DT>(p, t, s);
+        }
+    };
+    if (d_type == TYPE_F32) return go(float{});
+    return go(T{});
+}
+
+}  // namespace miw
