@@ -77,7 +77,7 @@ struct grouped_params {
     int vector;   // 16-byte accesses to the operands
     int d_vector; // aligned stores of four elements
 };
-enum grouped_tile_size { TILE_256x128, TILE_128x128, TILE_128x64 };
+enum grouped_tile_size { TILE_256x256, TILE_256x128, TILE_128x128, TILE_128x64 };
 hipError_t launch_grouped_tile_f16(const grouped_params &p, grouped_tile_size t, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_tile_bf16(const grouped_params &p, grouped_tile_size t, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_tile_mxfp4(const grouped_params &p, grouped_tile_size t, int d_type, hipStream_t s);

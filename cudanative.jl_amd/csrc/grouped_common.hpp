@@ -26,9 +26,20 @@ __device__ inline int source_row(const grouped_params &p, int position)
 // Tiles of BJ rows over all groups: a group has ceil(rows / BJ), and how many there are is only known on the device.
 // The launch has as many workgroups as there can be at most (rows / BJ + groups, times the tiles along i) and each
 // finds its own from the offsets: every wavefront sums the groups' tile counts 64 at a time, without LDS.
-// The tiles that there are go to the XCDs in eight runs, as in gemm_tiled.hpp; within a group eight tiles of rows (GJ) share
-// the way along i, so that an XCD's CUs read few panels of weights and few of rows at a time.
+// Within a group eight tiles of rows share the way along i, and an XCD's CUs take 32 tiles that follow one another, so that
+// they read few panels of weights and few of rows at a time.
 constexpr int GROUP_J_TILES = 8;
+// Workgroup -> tile, or -1.  Workgroups go round-robin over the eight XCDs; 256 tiles at a time are cut into eight runs.  (One run
+// of all tiles for each XCD gives it whole groups, and the XCD with the longest ones ends last: the gradient to the
+// weights of 16 uneven groups, 4096 x 2048 each, took 314 us like that.)
+__device__ inline int tile_of_workgroup(int total)
+{
+    const int xcd = (int)blockIdx.x & 7, loc = (int)blockIdx.x >> 3;
+    const int whole = total >> 8, rest = total & 255;
+    if (loc < whole * 32) return (loc >> 5) * 256 + xcd * 32 + (loc & 31);
+    const int run = (rest + 7) >> 3, at = loc - whole * 32, tile = xcd * run + at;
+    return at < run && tile < rest ? whole * 256 + tile : -1;
+}
 struct grouped_tile {
     int group, first, last, j0, i0;  // first, last: the group's rows; j0: first row of the tile; group -1: no tile
 };
@@ -45,10 +56,8 @@ __device__ inline grouped_tile find_tile(const grouped_params &p, int bi, int bj
     int total = __builtin_amdgcn_readlane(upto, 63);
     for (int g0 = 64; g0 < p.groups; g0 += 64) total += __builtin_amdgcn_readlane(wave_scan(count(g0 + lane)), 63);
     total = min(max(total, 0) * tiles_i, (int)gridDim.x);
-    int id = (int)blockIdx.x;
-    const int per = total >> 3, rem = total & 7, xcd = id & 7, loc = id >> 3;
-    if (loc >= per + (xcd < rem)) return {-1, 0, 0, 0, 0};
-    id = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+    int id = tile_of_workgroup(total);
+    if (id < 0) return {-1, 0, 0, 0, 0};
     const int row_tile = id / tiles_i;  // (of all groups; a group's tiles are numbered together)
     int g0 = 0, before = 0;
     unsigned long beyond = __ballot(upto > row_tile);
@@ -76,7 +85,8 @@ __device__ inline grouped_tile find_tile(const grouped_params &p, int bi, int bj
 // Workgroups of a launch over tiles of bi x bj, or 0 where they do not fit in a grid.
 inline long grouped_blocks(const grouped_params &p, long bi, long bj, long threads)
 {
-    const long n = (p.rows / bj + (p.groups < p.rows ? p.groups : p.rows)) * ((p.I + bi - 1) / bi);
+    const long tiles = (p.rows / bj + (p.groups < p.rows ? p.groups : p.rows)) * ((p.I + bi - 1) / bi);
+    const long n = (tiles + 7) / 8 * 8;  // (an XCD's share may be one more than a whole number of eighths)
     return n * threads < (1l << 32) && n < (1l << 30) ? n : 0;
 }
 
@@ -124,12 +134,13 @@ struct mfma_bf16 {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec<__bf16, 8>, x), __builtin_bit_cast(vec<__bf16, 8>, y), acc, 0, 0, 0);
     }
 };
-// 32 values of e2m1 a lane, with one scale each for its 32 of X and of Y in the low byte.
+// 32 values of e2m1 a lane, with one scale each for its 32 of X and of Y in byte BYTE.
+template <int BYTE>
 __device__ inline f32x4 mac_mxfp4(u32x4 x, u32x4 y, f32x4 acc, unsigned xs, unsigned ys)
 {
     typedef int i32x8 __attribute__((ext_vector_type(8)));
     const i32x8 a = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0}, b = {(int)y[0], (int)y[1], (int)y[2], (int)y[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4 /* e2m1 */, 4, 0, (int)xs, 0, (int)ys);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4 /* e2m1 */, 4, BYTE, (int)xs, BYTE, (int)ys);
 }
 
 }  // namespace miw

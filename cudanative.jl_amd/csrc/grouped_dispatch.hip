@@ -1,10 +1,12 @@
 // Which kernel runs a product grouped by expert.
 #include "experts.hpp"
+#include <cstdlib>
 
 namespace miw {
 
 static grouped_tile_size pick(const grouped_params &p)
 {
+    if (const char *e = getenv("MIW_TILE")) return (grouped_tile_size)atoi(e);
     return p.I > 128 && p.rows / p.groups > 64 ? TILE_256x128 : TILE_128x64;
 }
 

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64) void k_grouped_mxfp4_plain(grouped_params p)
             sx = xs[(long)(b / 8) * p.lxs * 8 + b % 8];
             sy = ys[(long)(b / 8) * p.lys * 8 + b % 8];
         }
-        acc = mac_mxfp4(xv, yv, acc, sx, sy);
+        acc = mac_mxfp4<0>(xv, yv, acc, sx, sy);
     }
     if (t.j0 + r < t.last) store_results<DT>(p, (DT *)p.D + (long)(t.j0 + r) * p.ldd, t.i0 + 4 * q, acc);
 }

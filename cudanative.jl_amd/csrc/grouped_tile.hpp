@@ -50,13 +50,12 @@ constexpr int grouped_lds_bytes(int bi, int bj, int nslot, bool scaled, int form
     return nslot * grouped_slot_bytes(bi, bj, scaled) + (form == RAGGED_SUM ? 2 * nslot * 256 : 0);
 }
 
-// Tile of a ragged sum: groups one after the other, in runs over the XCDs, eight tiles along j together.
+// Tile of a ragged sum: groups one after the other, eight tiles along j together.
 __device__ inline grouped_tile find_sum_tile(const grouped_params &p, int bi, int bj)
 {
     const int tiles_i = (p.I + bi - 1) / bi, tiles_j = (p.J + bj - 1) / bj;
-    int id = (int)blockIdx.x;
-    const int per = (int)gridDim.x >> 3, rem = (int)gridDim.x & 7, xcd = id & 7, loc = id >> 3;
-    id = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+    int id = tile_of_workgroup(p.groups * tiles_i * tiles_j);
+    if (id < 0) return {-1, 0, 0, 0, 0};
     const int group = id / (tiles_i * tiles_j);
     id -= group * tiles_i * tiles_j;
     const group_rows rows = rows_of_group(p, group);
@@ -84,10 +83,13 @@ void k_grouped_tile(grouped_params p)
     constexpr int WTI = BI / WI, WTJ = BJ / WJ, TI = WTI / 16, TJ = WTJ / 16;
     constexpr int XBYTES = BI * 128, YBYTES = BJ * 128, SLOT = grouped_slot_bytes(BI, BJ, SCALED);
     constexpr int XS = XBYTES + YBYTES, YS = XS + BI * 8, INDEX = NSLOT * SLOT;  // scales in the slot; the ring of gathered rows
-    static_assert(grouped_lds_bytes(BI, BJ, NSLOT, SCALED, FORM) <= 160 * 1024 && NSLOT >= 3, "ring does not fit in LDS");
-    constexpr int NLX = BI / 64, NLY = BJ / 64, EXTRA = SCALED ? 2 : SUM ? 1 : 0, LPAIR = NLX + NLY + EXTRA;
-    constexpr int NFRAG = 2 * (TI + TJ);
-    static_assert(BI % 128 == 0 && BJ % 64 == 0 && WTI % 16 == 0 && WTJ % 16 == 0, "tile");
+    static_assert(grouped_lds_bytes(BI, BJ, NSLOT, SCALED, FORM) <= 160 * 1024 && NSLOT >= 2, "ring does not fit in LDS");
+    constexpr bool HALVES = NSLOT == 2;  // a cluster is one MFMA step of the slot, otherwise both
+    constexpr int XSW = BI / 128, YSW = BJ / 32;  // wavefronts' loads that a slot's scales take
+    constexpr bool SHARED_SCALES = XSW + YSW <= 8;
+    constexpr int NLX = BI / 64, NLY = BJ / 64, EXTRA = SCALED ? (SHARED_SCALES ? 1 : 2) : SUM ? 1 : 0, LPAIR = NLX + NLY + EXTRA;
+    constexpr int NFRAG = (HALVES ? 1 : 2) * (TI + TJ);  // of a cluster
+    static_assert(BI % 128 == 0 && BJ % 64 == 0 && WTI % 32 == 0 && WTJ % 16 == 0, "tile");
 
     extern __shared__ __attribute__((aligned(128))) char smem[];
     MIW_LDS char *lds = (MIW_LDS char *)smem;
@@ -128,22 +130,25 @@ void k_grouped_tile(grouped_params p)
 #pragma unroll
         for (int i = 0; i < NLY; i++) yp[i] = Y + 2l * (at.j0 + min(64 * i + i_chunk * 8, p.J - 8 - at.j0));
     }
-    const int x_scale_wave = wave % (BI / 128), y_scale_wave = wave % (BJ / 32);
+    // Scales: X's are fetched 16 bytes (two rows) a lane, Y's, whose rows may lie anywhere, four bytes a lane.  Where the
+    // wavefronts suffice the first ones fetch X's and the others Y's, one load each; otherwise every one fetches a part of
+    // both.  All count the same: those that are left over repeat another's.
+    static_assert(!SCALED || (XSW <= 8 && YSW <= 8), "loads of scales");
+    const bool x_scales = SHARED_SCALES && wave < XSW;
+    const int x_part = wave % XSW, y_part = SHARED_SCALES ? (wave + YSW - XSW % YSW) % YSW : wave % YSW;
     const char *xsp = nullptr, *ysp = nullptr;
     if constexpr (SCALED) {
-        xsp = (const char *)p.xs + (long)at.group * p.sxs + 8l * min((long)at.i0 + x_scale_wave * 128 + 2 * lane, p.lxs - 2);
-        const int dword = y_scale_wave * 64 + lane;
+        xsp = (const char *)p.xs + (long)at.group * p.sxs + 8l * min((long)at.i0 + x_part * 128 + 2 * lane, p.lxs - 2);
+        const int dword = y_part * 64 + lane;
         ysp = (const char *)p.ys + 8l * source_row(p, min(at.j0 + (dword >> 1), at.last - 1)) + 4 * (dword & 1);
     }
-    const long x_step = XK ? 128 : 64 * p.ldx, xs_step = 8 * p.lxs, ys_step = 8 * p.lys;
+    const long x_step = XK ? 128 : 64 * p.ldx;
 
     const unsigned wave_dst = (unsigned)(uintptr_t)lds + (unsigned)wave * 1024u;
     const unsigned lds0 = (unsigned)(uintptr_t)lds;
     int next = 0;       // slot to request
     unsigned woff = 0;  // its place in the ring
-    unsigned xw = 0, yw = 0;  // (ragged sum: the lane's rows of the slot, in bytes from the operands)
-    long xrow = 0, yrow = 0;
-    (void)xw; (void)yw;
+    long xrow = 0, yrow = 0;  // (ragged sum: the lane's rows of the slot, in bytes from the operands)
     auto last_slot_begins = [&]() MIW_INLINE {
         if constexpr (XK) {
             const unsigned back = 16u * (unsigned)max(0, k_chunk - (last_chunks - 1));
@@ -178,8 +183,9 @@ void k_grouped_tile(grouped_params p)
             if constexpr (SUM) lds_load16<XBYTES + M * NT * 16>(yp[M] + yrow, dst);
             else lds_load16<XBYTES + M * NT * 16>(yp[M], dst);
         } else if constexpr (SCALED) {
-            if constexpr (N == NLX + NLY) lds_load16<XS>(xsp, lds0 + woff + (unsigned)x_scale_wave * 1024u);
-            else lds_load4<YS>(ysp, lds0 + woff + (unsigned)y_scale_wave * 256u);
+            const bool x_turn = SHARED_SCALES ? x_scales : N == NLX + NLY;
+            if (x_turn) lds_load16<XS>(xsp, lds0 + woff + (unsigned)x_part * 1024u);
+            else lds_load4<YS>(ysp, lds0 + woff + (unsigned)y_part * 256u);
         } else if constexpr (SUM) {
             // the rows of the slot NSLOT - 1 further on, by every wavefront to the same place
             const int position = min(at.first + min(next + NSLOT - 1, NP - 1) * 64 + lane, at.last - 1);
@@ -196,8 +202,8 @@ void k_grouped_tile(grouped_params p)
 #pragma unroll
             for (int i = 0; i < NLY; i++) yp[i] += 128;
             if constexpr (SCALED) {
-                xsp += xs_step;
-                ysp += ys_step;
+                xsp += 8 * p.lxs;
+                ysp += 8 * p.lys;
             }
             if (next == NP - 1) last_slot_begins();
         }
@@ -215,6 +221,7 @@ void k_grouped_tile(grouped_params p)
 
     if (NP > 0) {
         if (NP == 1) last_slot_begins();
+        // The first slots (a sum that is shorter than the ring asks for its last slot again, which nobody reads).
 #pragma unroll
         for (int s = 0; s < NSLOT - 1; s++) {
             if constexpr (SUM) find_rows(direct_row());
@@ -223,104 +230,142 @@ void k_grouped_tile(grouped_params p)
         }
         wait_loads_and_barrier<(NSLOT - 2) * LPAIR>();
 
-        u32x4 fx[2][TI], fy[2][TJ];
-        u32x2 sx[SCALED ? TI : 1], sy[SCALED ? TJ : 1];
+        constexpr int FSETS = HALVES ? 1 : 2;
+        u32x4 fx[FSETS][TI], fy[FSETS][TJ];
+        unsigned lane_sx[SCALED ? TI : 1], lane_sy[SCALED ? TJ : 1];  // this lane's scales of steps 0 and 1 in the low bytes
+        const unsigned own_bytes = (unsigned)(q | (4 + q) << 8 | 0x0c0c0000);
+        (void)own_bytes;
         unsigned roff = 0;
-        auto cluster_unit = [&]<int U>(MIW_LDS const char *slot, std::integral_constant<int, U>) MIW_INLINE {
-            [&]<int... N>(std::integer_sequence<int, N...>) {
-                (([&] {
-                     if constexpr (N * NFRAG / LPAIR == U) {
-                         request_one(std::integral_constant<int, N>{});
-                         __builtin_amdgcn_sched_barrier(0);
-                     }
-                 }()),
-                 ...);
-            }(std::make_integer_sequence<int, LPAIR>{});
-            constexpr int H = U / (TI + TJ), V = U % (TI + TJ);
-            if constexpr (V < TI) fx[H][V] = __builtin_bit_cast(u32x4, xr.template read<V, H>(slot));
-            else fy[H][V - TI] = __builtin_bit_cast(u32x4, yr.template read<V - TI, H>(slot + XBYTES));
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        auto memory_cluster = [&]() MIW_INLINE {
+        constexpr std::integral_constant<int, 0> step0{};
+        constexpr std::integral_constant<int, 1> step1{};
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        // Memory cluster H (of one: 0): its fragments, and with REQUEST the loads of the slot NSLOT - 1 further on, all in cluster
+        // 0, at even distances between the reads.  REQUEST is false where the sum has no such slot.
+        auto memory_cluster = [&]<int H, bool REQUEST>(std::integral_constant<int, H>, std::bool_constant<REQUEST>) MIW_INLINE {
+            constexpr bool FIRST = H == 0, LAST = !HALVES || H == 1;
             MIW_LDS const char *slot = lds + roff;
-            if constexpr (SUM) {
+            if constexpr (SUM && FIRST && REQUEST) {
                 const int row = p.gather ? min(max(*(MIW_LDS const int *)(lds + INDEX + index_entry(next) + 4 * line), 0), p.source_rows - 1)
                                          : min(at.first + next * 64 + line, at.last - 1);
                 find_rows(row);
             }
-            if constexpr (SCALED) {
+            u32x2 sx[SCALED ? TI : 1], sy[SCALED ? TJ : 1];  // a row's eight scales of the slot
+            if constexpr (SCALED && FIRST) {
 #pragma unroll
                 for (int a = 0; a < TI; a++) sx[a] = *(MIW_LDS const u32x2 *)(slot + XS + (wi * WTI + 16 * a + r) * 8);
 #pragma unroll
                 for (int b = 0; b < TJ; b++) sy[b] = *(MIW_LDS const u32x2 *)(slot + YS + (wj * WTJ + 16 * b + r) * 8);
             }
-            [&]<int... U>(std::integer_sequence<int, U...>) { (cluster_unit(slot, std::integral_constant<int, U>{}), ...); }(std::make_integer_sequence<int, NFRAG>{});
-            end_request();
-            roff = roff + SLOT == NSLOT * SLOT ? 0 : roff + SLOT;
+            auto unit = [&]<int U>(std::integral_constant<int, U>) MIW_INLINE {
+                if constexpr (FIRST && REQUEST)
+                    [&]<int... N>(std::integer_sequence<int, N...>) {
+                        (([&] {
+                             if constexpr (N * NFRAG / LPAIR == U) {
+                                 request_one(std::integral_constant<int, N>{});
+                                 __builtin_amdgcn_sched_barrier(0);
+                             }
+                         }()),
+                         ...);
+                    }(std::make_integer_sequence<int, LPAIR>{});
+                constexpr int S = HALVES ? 0 : U / (TI + TJ), T = HALVES ? H : S, V = U % (TI + TJ);
+                if constexpr (V < TI) fx[S][V] = __builtin_bit_cast(u32x4, xr.template read<V, T>(slot));
+                else fy[S][V - TI] = __builtin_bit_cast(u32x4, yr.template read<V - TI, T>(slot + XBYTES));
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            [&]<int... U>(std::integer_sequence<int, U...>) { (unit(std::integral_constant<int, U>{}), ...); }(std::make_integer_sequence<int, NFRAG>{});
+            if constexpr (FIRST && REQUEST) end_request();
+            if constexpr (LAST) roff = roff + SLOT == NSLOT * SLOT ? 0 : roff + SLOT;
+            if constexpr (SCALED && FIRST) {
+#pragma unroll
+                for (int a = 0; a < TI; a++) lane_sx[a] = __builtin_amdgcn_perm(sx[a][1], sx[a][0], own_bytes);
+#pragma unroll
+                for (int b = 0; b < TJ; b++) lane_sy[b] = __builtin_amdgcn_perm(sy[b][1], sy[b][0], own_bytes);
+            }
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto compute_cluster = [&]() MIW_INLINE {
+        auto multiply = [&]<int S, int T>(std::integral_constant<int, S>, std::integral_constant<int, T>) MIW_INLINE {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int m = 0; m < TI * TJ; m++) {
-                    const int a = m / TJ, b = serpentine_column(m, TJ);
-                    if constexpr (SCALED) acc[a][b] = mac_mxfp4(fx[h][a], fy[h][b], acc[a][b], sx[a][h] >> (8 * q), sy[b][h] >> (8 * q));
-                    else acc[a][b] = OP::mac(fx[h][a], fy[h][b], acc[a][b]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-        };
-        // Zeroes what the last slot's lanes fetched again; a block's scale that goes with it becomes 1.
-        auto mask_tail = [&]() MIW_INLINE {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (SCALED) {
-                    const bool in = 4 * h + q < last_chunks;
-#pragma unroll
-                    for (int a = 0; a < TI; a++) {
-                        if (!in) fx[h][a] = u32x4{0, 0, 0, 0};
-                        sx[a][h] = in ? sx[a][h] : 0x7f7f7f7fu;
-                    }
-#pragma unroll
-                    for (int b = 0; b < TJ; b++) {
-                        if (!in) fy[h][b] = u32x4{0, 0, 0, 0};
-                        sy[b][h] = in ? sy[b][h] : 0x7f7f7f7fu;
-                    }
-                } else {
-                    const int keep = last_values - (32 * h + 8 * q);
-#pragma unroll
-                    for (int a = 0; a < TI; a++) keep_first(fx[h][a], keep);
-#pragma unroll
-                    for (int b = 0; b < TJ; b++) keep_first(fy[h][b], keep);
-                }
+            for (int m = 0; m < TI * TJ; m++) {
+                const int a = m / TJ, b = serpentine_column(m, TJ);
+                if constexpr (SCALED) acc[a][b] = mac_mxfp4<T>(fx[S][a], fy[S][b], acc[a][b], lane_sx[a], lane_sy[b]);
+                else acc[a][b] = OP::mac(fx[S][a], fy[S][b], acc[a][b]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (late_group) __builtin_amdgcn_s_barrier();
-        for (int s = 0; s < NP - 1; s++) {
-            memory_cluster();
-            wait_loads_and_barrier<(NSLOT - 2) * LPAIR>();
-            compute_cluster();
+        // Zeroes what the last slot's lanes fetched again; a block's scale that goes with it becomes 1.
+        auto mask_tail = [&]<int S, int T>(std::integral_constant<int, S>, std::integral_constant<int, T>) MIW_INLINE {
+            if constexpr (SCALED) {
+                const bool in = 4 * T + q < last_chunks;
+                constexpr unsigned one = 0x7fu << (8 * T), others = ~(0xffu << (8 * T));
+#pragma unroll
+                for (int a = 0; a < TI; a++) {
+                    if (!in) fx[S][a] = u32x4{0, 0, 0, 0};
+                    if (!in) lane_sx[a] = (lane_sx[a] & others) | one;
+                }
+#pragma unroll
+                for (int b = 0; b < TJ; b++) {
+                    if (!in) fy[S][b] = u32x4{0, 0, 0, 0};
+                    if (!in) lane_sy[b] = (lane_sy[b] & others) | one;
+                }
+            } else {
+                const int keep = last_values - (32 * T + 8 * q);
+#pragma unroll
+                for (int a = 0; a < TI; a++) keep_first(fx[S][a], keep);
+#pragma unroll
+                for (int b = 0; b < TJ; b++) keep_first(fy[S][b], keep);
+            }
+        };
+        // One slot.  At the end of its last memory cluster the wavefront lets the NSLOT - 2 youngest slots stay in flight (none where
+        // the sum's last ones are being used up): the next slot has landed, and the barriers that follow publish it.
+        auto one_slot = [&]<bool REQUEST, bool MASK>(std::bool_constant<REQUEST> request, std::bool_constant<MASK>) MIW_INLINE {
+            constexpr int INFLIGHT = REQUEST ? (NSLOT - 2) * LPAIR : 0;
+            memory_cluster(step0, request);
+            if constexpr (HALVES) {
+                wait_loads_and_barrier<63>();  // (the fragments alone)
+                if constexpr (MASK) mask_tail(step0, step0);
+                multiply(step0, step0);
+                __builtin_amdgcn_s_barrier();
+                memory_cluster(step1, request);
+                wait_loads_and_barrier<INFLIGHT>();
+                if constexpr (MASK) mask_tail(step0, step1);
+                multiply(step0, step1);
+            } else {
+                wait_loads_and_barrier<INFLIGHT>();
+                if constexpr (MASK) {
+                    mask_tail(step0, step0);
+                    mask_tail(step1, step1);
+                }
+                multiply(step0, step0);
+                multiply(step1, step1);
+            }
             __builtin_amdgcn_s_barrier();
-        }
-        memory_cluster();
-        wait_loads_and_barrier<(NSLOT - 2) * LPAIR>();
-        mask_tail();
-        compute_cluster();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may outlive the workgroup's LDS
+        };
+        if (late_group) __builtin_amdgcn_s_barrier();
+        int s = 0;
+        for (; s < NP - (NSLOT - 1); s++) one_slot(yes, no);
+        for (; s < NP - 1; s++) one_slot(no, no);
+        one_slot(no, yes);
         if (!late_group) __builtin_amdgcn_s_barrier();
     }
 
+    // Neighbouring lanes hold neighbouring rows: they exchange the results of two MFMA tiles, so that a row's 32 go out together
+    // (128 bytes of Float32) from eight lanes, first the even rows and then the odd ones.
     DT *D = (DT *)p.D + (SUM ? (long)at.group * p.sd : 0);
     const int end_j = SUM ? p.J : at.last;
+    const bool odd = r & 1;
 #pragma unroll
     for (int b = 0; b < TJ; b++) {
-        const int j = at.j0 + wj * WTJ + 16 * b + r;
-        if (j < end_j) {
-            DT *row = D + (long)j * p.ldd;
+        const int j = at.j0 + wj * WTJ + 16 * b + (r & ~1);
+        DT *row = D + (long)j * p.ldd;
 #pragma unroll
-            for (int a = 0; a < TI; a++) store_results<DT>(p, row, at.i0 + wi * WTI + 16 * a + 4 * q, acc[a][b]);
+        for (int a = 0; a < TI; a += 2) {
+            float4_t v0 = acc[a][b], v1 = acc[a + 1][b];
+            pair_exchange(odd, v0, v1);
+            const int i = at.i0 + wi * WTI + 16 * (a + odd) + 4 * q;
+            if (j < end_j) store_results<DT>(p, row, i, v0);
+            if (j + 1 < end_j) store_results<DT>(p, row + p.ldd, i, v1);
         }
     }
 }
