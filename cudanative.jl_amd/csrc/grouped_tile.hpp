@@ -44,10 +44,11 @@ __device__ inline void lds_load4(const char *lane_address, unsigned lds_base)
     asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_base), "v"(lane_address), "n"(DST) : "memory", "m0", "scc");
 }
 
-constexpr int grouped_slot_bytes(int bi, int bj, bool scaled) { return (bi + bj) * (128 + (scaled ? 8 : 0)); }
-constexpr int grouped_lds_bytes(int bi, int bj, int nslot, bool scaled, int form)
+// A slot of one operand: its rows' 128 bytes, then their scales.
+constexpr int grouped_slot_bytes(int rows, bool scaled) { return rows * (128 + (scaled ? 8 : 0)); }
+constexpr int grouped_lds_bytes(int bi, int bj, int nx, int ny, bool scaled, int form)
 {
-    return nslot * grouped_slot_bytes(bi, bj, scaled) + (form == RAGGED_SUM ? 2 * nslot * 256 : 0);
+    return nx * grouped_slot_bytes(bi, scaled) + ny * grouped_slot_bytes(bj, scaled) + (form == RAGGED_SUM ? 2 * ny * 256 : 0);
 }
 
 // Tile of a ragged sum: groups one after the other, eight tiles along j together.
@@ -72,7 +73,13 @@ __device__ inline void keep_first(u32x4 &f, int keep)
     for (int e = 0; e < 4; e++) f[e] &= keep >= 2 * e + 2 ? 0xffffffffu : keep == 2 * e + 1 ? 0xffffu : 0u;
 }
 
-template <class OP, int BI, int BJ, int WI, int WJ, int NSLOT, int FORM, class DT>
+// NX, NY: slots of X and of Y in LDS.
+//   Three or more, as many of both: a cluster is a whole slot.  The slot NX - 1 further on is requested in a slot's memory
+//     cluster, into the place of the one before, and at its end the NX - 2 youngest stay in flight.
+//   Two of Y (tiles of 256 x 256): a cluster is one MFMA step, half a slot.  Y's next slot is requested in the first memory cluster and
+//     has to have landed at the end of the second; X's goes with it, or, with three slots of X, the one after that in the
+//     second cluster, so that X, the weights, which come from HBM where the rows mostly come from caches, has twice the time.
+template <class OP, int BI, int BJ, int WI, int WJ, int NX, int NY, int FORM, class DT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void k_grouped_tile(grouped_params p)
 {
@@ -81,13 +88,15 @@ void k_grouped_tile(grouped_params p)
     constexpr bool XK = FORM == ROWS_X_K, YK = FORM != RAGGED_SUM, SUM = FORM == RAGGED_SUM, SCALED = OP::scaled;
     static_assert(!SCALED || XK, "4-bit operands have k contiguous");
     constexpr int WTI = BI / WI, WTJ = BJ / WJ, TI = WTI / 16, TJ = WTJ / 16;
-    constexpr int XBYTES = BI * 128, YBYTES = BJ * 128, SLOT = grouped_slot_bytes(BI, BJ, SCALED);
-    constexpr int XS = XBYTES + YBYTES, YS = XS + BI * 8, INDEX = NSLOT * SLOT;  // scales in the slot; the ring of gathered rows
-    static_assert(grouped_lds_bytes(BI, BJ, NSLOT, SCALED, FORM) <= 160 * 1024 && NSLOT >= 2, "ring does not fit in LDS");
-    constexpr bool HALVES = NSLOT == 2;  // a cluster is one MFMA step of the slot, otherwise both
+    constexpr int XBYTES = BI * 128, YBYTES = BJ * 128, XSLOT = grouped_slot_bytes(BI, SCALED), YSLOT = grouped_slot_bytes(BJ, SCALED);
+    constexpr int XRING = NX * XSLOT, YRING = NY * YSLOT, INDEX = XRING + YRING;  // X's ring, Y's, that of the gathered rows
+    static_assert(grouped_lds_bytes(BI, BJ, NX, NY, SCALED, FORM) <= 160 * 1024, "rings do not fit in LDS");
+    constexpr bool HALVES = NY == 2, SPLIT = HALVES && NX == 3;
+    static_assert(SPLIT ? !SCALED && !SUM : NX == NY, "slots");
     constexpr int XSW = BI / 128, YSW = BJ / 32;  // wavefronts' loads that a slot's scales take
     constexpr bool SHARED_SCALES = XSW + YSW <= 8;
-    constexpr int NLX = BI / 64, NLY = BJ / 64, EXTRA = SCALED ? (SHARED_SCALES ? 1 : 2) : SUM ? 1 : 0, LPAIR = NLX + NLY + EXTRA;
+    constexpr int NLX = BI / 64, NLY = BJ / 64, EXTRA = SCALED ? (SHARED_SCALES ? 1 : 2) : SUM ? 1 : 0;
+    constexpr int LPAIR = NLX + NLY + EXTRA;  // loads a thread and slot
     constexpr int NFRAG = (HALVES ? 1 : 2) * (TI + TJ);  // of a cluster
     static_assert(BI % 128 == 0 && BJ % 64 == 0 && WTI % 32 == 0 && WTJ % 16 == 0, "tile");
 
@@ -146,66 +155,74 @@ void k_grouped_tile(grouped_params p)
 
     const unsigned wave_dst = (unsigned)(uintptr_t)lds + (unsigned)wave * 1024u;
     const unsigned lds0 = (unsigned)(uintptr_t)lds;
-    int next = 0;       // slot to request
-    unsigned woff = 0;  // its place in the ring
-    long xrow = 0, yrow = 0;  // (ragged sum: the lane's rows of the slot, in bytes from the operands)
-    auto last_slot_begins = [&]() MIW_INLINE {
-        if constexpr (XK) {
-            const unsigned back = 16u * (unsigned)max(0, k_chunk - (last_chunks - 1));
+    int xnext = 0, ynext = 0;    // slots to request (one number, ynext, without SPLIT)
+    unsigned xwoff = 0, ywoff = 0;  // their places in the rings
+    long xrow = 0, yrow = 0;     // (ragged sum: the lane's rows of the slot, in bytes from the operands)
+    auto x_last_begins = [&]() MIW_INLINE {
+        if constexpr (SUM) return;
+        const unsigned back = XK ? 16u * (unsigned)max(0, k_chunk - (last_chunks - 1)) : (unsigned)(max(0, line - (last_values - 1)) * (int)p.ldx);
 #pragma unroll
-            for (int i = 0; i < NLX; i++) xvo[i] -= back;
-        } else if constexpr (!SUM) {
-            const unsigned back = (unsigned)(max(0, line - (last_values - 1)) * (int)p.ldx);
-#pragma unroll
-            for (int i = 0; i < NLX; i++) xvo[i] -= back;
-        }
-        if constexpr (YK) {
-            const int back = 16 * max(0, k_chunk - (last_chunks - 1));
-#pragma unroll
-            for (int i = 0; i < NLY; i++) yp[i] -= back;
-        }
+        for (int i = 0; i < NLX; i++) xvo[i] -= back;
     };
-    // Ragged sum: where this lane's row of slot `next` lies in both operands.
+    auto y_last_begins = [&]() MIW_INLINE {
+        if constexpr (SUM) return;
+        const int back = 16 * max(0, k_chunk - (last_chunks - 1));
+#pragma unroll
+        for (int i = 0; i < NLY; i++) yp[i] -= back;
+    };
+    // Ragged sum: where this lane's row of slot `ynext` lies in both operands.
     auto find_rows = [&](int gathered) MIW_INLINE {
-        const int position = min(at.first + next * 64 + line, at.last - 1);
+        const int position = min(at.first + ynext * 64 + line, at.last - 1);
         yrow = (long)position * p.ldy;
         xrow = (long)gathered * p.ldx;
     };
-    auto direct_row = [&]() MIW_INLINE { return source_row(p, min(at.first + next * 64 + line, at.last - 1)); };
-    auto index_entry = [&](int slot) MIW_INLINE { return (unsigned)(slot % (2 * NSLOT)) * 256u; };
+    auto direct_row = [&]() MIW_INLINE { return source_row(p, min(at.first + ynext * 64 + line, at.last - 1)); };
+    auto index_entry = [&](int slot) MIW_INLINE { return (unsigned)(slot % (2 * NY)) * 256u; };
+    // Load N of a slot: X's, Y's, then what goes with them.
     auto request_one = [&]<int N>(std::integral_constant<int, N>) MIW_INLINE {
-        const unsigned dst = wave_dst + woff;
         if constexpr (N < NLX) {
+            const unsigned dst = wave_dst + xwoff;
             if constexpr (SUM) lds_load16<N * NT * 16>(X + xvo[N] + xrow, dst);
             else lds_dma16_at<N * NT * 16, 0>(X, xvo[N], dst);
         } else if constexpr (N < NLX + NLY) {
             constexpr int M = N - NLX;
-            if constexpr (SUM) lds_load16<XBYTES + M * NT * 16>(yp[M] + yrow, dst);
-            else lds_load16<XBYTES + M * NT * 16>(yp[M], dst);
+            const unsigned dst = wave_dst + ywoff;
+            if constexpr (SUM) lds_load16<XRING + M * NT * 16>(yp[M] + yrow, dst);
+            else lds_load16<XRING + M * NT * 16>(yp[M], dst);
         } else if constexpr (SCALED) {
             const bool x_turn = SHARED_SCALES ? x_scales : N == NLX + NLY;
-            if (x_turn) lds_load16<XS>(xsp, lds0 + woff + (unsigned)x_part * 1024u);
-            else lds_load4<YS>(ysp, lds0 + woff + (unsigned)y_part * 256u);
+            if (x_turn) lds_load16<XBYTES>(xsp, lds0 + xwoff + (unsigned)x_part * 1024u);
+            else lds_load4<XRING + YBYTES>(ysp, lds0 + ywoff + (unsigned)y_part * 256u);
         } else if constexpr (SUM) {
-            // the rows of the slot NSLOT - 1 further on, by every wavefront to the same place
-            const int position = min(at.first + min(next + NSLOT - 1, NP - 1) * 64 + lane, at.last - 1);
-            lds_load4<INDEX>((const char *)(p.gather ? p.gather + position : p.offsets), lds0 + index_entry(next + NSLOT - 1));
+            // the rows of the slot NY - 1 further on, by every wavefront to the same place
+            const int position = min(at.first + min(ynext + NY - 1, NP - 1) * 64 + lane, at.last - 1);
+            lds_load4<INDEX>((const char *)(p.gather ? p.gather + position : p.offsets), lds0 + index_entry(ynext + NY - 1));
         }
     };
-    auto end_request = [&]() MIW_INLINE {
-        woff = woff + SLOT == NSLOT * SLOT ? 0 : woff + SLOT;
+    // FROM .. TO - 1, in one go.
+    auto request_all = [&]<int FROM, int TO>(std::integral_constant<int, FROM>, std::integral_constant<int, TO>) MIW_INLINE {
+        [&]<int... I>(std::integer_sequence<int, I...>) { (request_one(std::integral_constant<int, FROM + I>{}), ...); }(std::make_integer_sequence<int, TO - FROM>{});
+    };
+    auto x_end_request = [&]() MIW_INLINE {
+        xwoff = xwoff + XSLOT == XRING ? 0 : xwoff + XSLOT;
+        if constexpr (!SUM)
+            if (xnext < NP - 1) {
+                xnext++;
+                X += x_step;
+                if constexpr (SCALED) xsp += 8 * p.lxs;
+                if (xnext == NP - 1) x_last_begins();
+            }
+    };
+    auto y_end_request = [&]() MIW_INLINE {
+        ywoff = ywoff + YSLOT == YRING ? 0 : ywoff + YSLOT;
         if constexpr (SUM) {
-            next++;
-        } else if (next < NP - 1) {
-            next++;
-            X += x_step;
+            ynext++;
+        } else if (ynext < NP - 1) {
+            ynext++;
 #pragma unroll
             for (int i = 0; i < NLY; i++) yp[i] += 128;
-            if constexpr (SCALED) {
-                xsp += 8 * p.lxs;
-                ysp += 8 * p.lys;
-            }
-            if (next == NP - 1) last_slot_begins();
+            if constexpr (SCALED) ysp += 8 * p.lys;
+            if (ynext == NP - 1) y_last_begins();
         }
     };
 
@@ -220,62 +237,81 @@ void k_grouped_tile(grouped_params p)
         for (int b = 0; b < TJ; b++) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     if (NP > 0) {
-        if (NP == 1) last_slot_begins();
-        // The first slots (a sum that is shorter than the ring asks for its last slot again, which nobody reads).
-#pragma unroll
-        for (int s = 0; s < NSLOT - 1; s++) {
-            if constexpr (SUM) find_rows(direct_row());
-            [&]<int... I>(std::integer_sequence<int, I...>) { (request_one(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, LPAIR>{});
-            end_request();
+        if (NP == 1) {
+            x_last_begins();
+            y_last_begins();
         }
-        wait_loads_and_barrier<(NSLOT - 2) * LPAIR>();
+        // The first slots (a sum that is shorter than the rings asks for its last slot again, which nobody reads).
+        constexpr std::integral_constant<int, 0> first_load{};
+        constexpr std::integral_constant<int, NLX> x_loads{};
+        constexpr std::integral_constant<int, LPAIR> all_loads{};
+#pragma unroll
+        for (int s = 0; s < NY - 1; s++) {
+            if constexpr (SUM) find_rows(direct_row());
+            request_all(first_load, all_loads);
+            x_end_request();
+            y_end_request();
+        }
+        if constexpr (SPLIT) {
+            request_all(first_load, x_loads);
+            x_end_request();
+            wait_loads_and_barrier<NLX>();
+        } else {
+            wait_loads_and_barrier<(NY - 2) * LPAIR>();
+        }
 
         constexpr int FSETS = HALVES ? 1 : 2;
         u32x4 fx[FSETS][TI], fy[FSETS][TJ];
         unsigned lane_sx[SCALED ? TI : 1], lane_sy[SCALED ? TJ : 1];  // this lane's scales of steps 0 and 1 in the low bytes
         const unsigned own_bytes = (unsigned)(q | (4 + q) << 8 | 0x0c0c0000);
         (void)own_bytes;
-        unsigned roff = 0;
+        unsigned xroff = 0, yroff = 0;  // the slot that is read, in the rings
         constexpr std::integral_constant<int, 0> step0{};
         constexpr std::integral_constant<int, 1> step1{};
         constexpr std::true_type yes{};
         constexpr std::false_type no{};
-        // Memory cluster H (of one: 0): its fragments, and with REQUEST the loads of the slot NSLOT - 1 further on, all in cluster
-        // 0, at even distances between the reads.  REQUEST is false where the sum has no such slot.
-        auto memory_cluster = [&]<int H, bool REQUEST>(std::integral_constant<int, H>, std::bool_constant<REQUEST>) MIW_INLINE {
+        // Memory cluster H (of one: 0): its fragments, and its requests at even distances between the reads.  REQUEST_X, REQUEST_Y:
+        // whether the sum has the slots that are next.
+        auto memory_cluster = [&]<int H, bool REQUEST_X, bool REQUEST_Y>(std::integral_constant<int, H>, std::bool_constant<REQUEST_X>,
+                                                                         std::bool_constant<REQUEST_Y>) MIW_INLINE {
             constexpr bool FIRST = H == 0, LAST = !HALVES || H == 1;
-            MIW_LDS const char *slot = lds + roff;
-            if constexpr (SUM && FIRST && REQUEST) {
-                const int row = p.gather ? min(max(*(MIW_LDS const int *)(lds + INDEX + index_entry(next) + 4 * line), 0), p.source_rows - 1)
-                                         : min(at.first + next * 64 + line, at.last - 1);
+            constexpr bool X_HERE = REQUEST_X && (SPLIT ? H == 1 : H == 0), Y_HERE = REQUEST_Y && H == 0;
+            constexpr int FROM = X_HERE ? 0 : NLX, TO = Y_HERE ? LPAIR : X_HERE ? NLX : FROM, COUNT = TO - FROM;
+            MIW_LDS const char *xs = lds + xroff, *ys = lds + XRING + yroff;
+            if constexpr (SUM && Y_HERE) {
+                const int row = p.gather ? min(max(*(MIW_LDS const int *)(lds + INDEX + index_entry(ynext) + 4 * line), 0), p.source_rows - 1)
+                                         : min(at.first + ynext * 64 + line, at.last - 1);
                 find_rows(row);
             }
             u32x2 sx[SCALED ? TI : 1], sy[SCALED ? TJ : 1];  // a row's eight scales of the slot
             if constexpr (SCALED && FIRST) {
 #pragma unroll
-                for (int a = 0; a < TI; a++) sx[a] = *(MIW_LDS const u32x2 *)(slot + XS + (wi * WTI + 16 * a + r) * 8);
+                for (int a = 0; a < TI; a++) sx[a] = *(MIW_LDS const u32x2 *)(xs + XBYTES + (wi * WTI + 16 * a + r) * 8);
 #pragma unroll
-                for (int b = 0; b < TJ; b++) sy[b] = *(MIW_LDS const u32x2 *)(slot + YS + (wj * WTJ + 16 * b + r) * 8);
+                for (int b = 0; b < TJ; b++) sy[b] = *(MIW_LDS const u32x2 *)(ys + YBYTES + (wj * WTJ + 16 * b + r) * 8);
             }
             auto unit = [&]<int U>(std::integral_constant<int, U>) MIW_INLINE {
-                if constexpr (FIRST && REQUEST)
-                    [&]<int... N>(std::integer_sequence<int, N...>) {
-                        (([&] {
-                             if constexpr (N * NFRAG / LPAIR == U) {
-                                 request_one(std::integral_constant<int, N>{});
-                                 __builtin_amdgcn_sched_barrier(0);
-                             }
-                         }()),
-                         ...);
-                    }(std::make_integer_sequence<int, LPAIR>{});
+                [&]<int... N>(std::integer_sequence<int, N...>) {
+                    (([&] {
+                         if constexpr (N * NFRAG / (COUNT ? COUNT : 1) == U) {
+                             request_one(std::integral_constant<int, FROM + N>{});
+                             __builtin_amdgcn_sched_barrier(0);
+                         }
+                     }()),
+                     ...);
+                }(std::make_integer_sequence<int, COUNT>{});
                 constexpr int S = HALVES ? 0 : U / (TI + TJ), T = HALVES ? H : S, V = U % (TI + TJ);
-                if constexpr (V < TI) fx[S][V] = __builtin_bit_cast(u32x4, xr.template read<V, T>(slot));
-                else fy[S][V - TI] = __builtin_bit_cast(u32x4, yr.template read<V - TI, T>(slot + XBYTES));
+                if constexpr (V < TI) fx[S][V] = __builtin_bit_cast(u32x4, xr.template read<V, T>(xs));
+                else fy[S][V - TI] = __builtin_bit_cast(u32x4, yr.template read<V - TI, T>(ys));
                 __builtin_amdgcn_sched_barrier(0);
             };
             [&]<int... U>(std::integer_sequence<int, U...>) { (unit(std::integral_constant<int, U>{}), ...); }(std::make_integer_sequence<int, NFRAG>{});
-            if constexpr (FIRST && REQUEST) end_request();
-            if constexpr (LAST) roff = roff + SLOT == NSLOT * SLOT ? 0 : roff + SLOT;
+            if constexpr (X_HERE) x_end_request();
+            if constexpr (Y_HERE) y_end_request();
+            if constexpr (LAST) {
+                xroff = xroff + XSLOT == XRING ? 0 : xroff + XSLOT;
+                yroff = yroff + YSLOT == YRING ? 0 : yroff + YSLOT;
+            }
             if constexpr (SCALED && FIRST) {
 #pragma unroll
                 for (int a = 0; a < TI; a++) lane_sx[a] = __builtin_amdgcn_perm(sx[a][1], sx[a][0], own_bytes);
@@ -317,17 +353,18 @@ void k_grouped_tile(grouped_params p)
                 for (int b = 0; b < TJ; b++) keep_first(fy[S][b], keep);
             }
         };
-        // One slot.  At the end of its last memory cluster the wavefront lets the NSLOT - 2 youngest slots stay in flight (none where
-        // the sum's last ones are being used up): the next slot has landed, and the barriers that follow publish it.
-        auto one_slot = [&]<bool REQUEST, bool MASK>(std::bool_constant<REQUEST> request, std::bool_constant<MASK>) MIW_INLINE {
-            constexpr int INFLIGHT = REQUEST ? (NSLOT - 2) * LPAIR : 0;
-            memory_cluster(step0, request);
+        // One slot.  At the end of its last memory cluster the next slot's loads have landed, what is younger stays in flight, and
+        // the barriers that follow publish them.
+        auto one_slot = [&]<bool REQUEST_X, bool REQUEST_Y, bool MASK>(std::bool_constant<REQUEST_X> want_x, std::bool_constant<REQUEST_Y> want_y,
+                                                                       std::bool_constant<MASK>) MIW_INLINE {
+            constexpr int INFLIGHT = SPLIT ? (REQUEST_X ? NLX : 0) : REQUEST_Y ? (NY - 2) * LPAIR : 0;
+            memory_cluster(step0, want_x, want_y);
             if constexpr (HALVES) {
                 wait_loads_and_barrier<63>();  // (the fragments alone)
                 if constexpr (MASK) mask_tail(step0, step0);
                 multiply(step0, step0);
                 __builtin_amdgcn_s_barrier();
-                memory_cluster(step1, request);
+                memory_cluster(step1, want_x, want_y);
                 wait_loads_and_barrier<INFLIGHT>();
                 if constexpr (MASK) mask_tail(step0, step1);
                 multiply(step0, step1);
@@ -344,9 +381,15 @@ void k_grouped_tile(grouped_params p)
         };
         if (late_group) __builtin_amdgcn_s_barrier();
         int s = 0;
-        for (; s < NP - (NSLOT - 1); s++) one_slot(yes, no);
-        for (; s < NP - 1; s++) one_slot(no, no);
-        one_slot(no, yes);
+        for (; s < NP - (NX - 1); s++) one_slot(yes, yes, no);
+        if constexpr (SPLIT) {
+            if (s < NP - 1) {
+                one_slot(no, yes, no);
+                s++;
+            }
+        }
+        for (; s < NP - 1; s++) one_slot(no, no, no);
+        one_slot(no, no, yes);
         if (!late_group) __builtin_amdgcn_s_barrier();
     }
 

@@ -6,16 +6,16 @@
 
 namespace miw {
 
-template <class OP, int BI, int BJ, int WI, int WJ, int NSLOT, int FORM, class DT>
+template <class OP, int BI, int BJ, int WI, int WJ, int NX, int NY, int FORM, class DT>
 static hipError_t launch_tile_instance(const grouped_params &p, hipStream_t s)
 {
-    constexpr int lds = grouped_lds_bytes(BI, BJ, NSLOT, OP::scaled, FORM);
-    const void *fn = (const void *)k_grouped_tile<OP, BI, BJ, WI, WJ, NSLOT, FORM, DT>;
+    constexpr int lds = grouped_lds_bytes(BI, BJ, NX, NY, OP::scaled, FORM);
+    const void *fn = (const void *)k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>;
     static const hipError_t allowed = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (allowed != hipSuccess) return allowed;
     const long blocks = FORM == RAGGED_SUM ? ((long)p.groups * ((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ) + 7) / 8 * 8 : grouped_blocks(p, BI, BJ, 512);
     if (blocks <= 0 || blocks >= 1l << 23) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((k_grouped_tile<OP, BI, BJ, WI, WJ, NSLOT, FORM, DT>), dim3((unsigned)blocks), dim3(512), lds, s, p);
+    hipLaunchKernelGGL((k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>), dim3((unsigned)blocks), dim3(512), lds, s, p);
     return hipGetLastError();
 }
 
@@ -23,10 +23,10 @@ template <class OP, int FORM, class DT>
 static hipError_t launch_tile_size(const grouped_params &p, grouped_tile_size t, hipStream_t s)
 {
     switch (t) {
-    case TILE_256x256: return launch_tile_instance<OP, 256, 256, 2, 4, 2, FORM, DT>(p, s);
-    case TILE_256x128: return launch_tile_instance<OP, 256, 128, 4, 2, 3, FORM, DT>(p, s);
-    case TILE_128x128: return launch_tile_instance<OP, 128, 128, 4, 2, 4, FORM, DT>(p, s);
-    default: return launch_tile_instance<OP, 128, 64, 4, 2, 6, FORM, DT>(p, s);
+    case TILE_256x256: return launch_tile_instance<OP, 256, 256, 2, 4, OP::scaled || FORM == RAGGED_SUM ? 2 : 3, 2, FORM, DT>(p, s);
+    case TILE_256x128: return launch_tile_instance<OP, 256, 128, 4, 2, 3, 3, FORM, DT>(p, s);
+    case TILE_128x128: return launch_tile_instance<OP, 128, 128, 4, 2, 4, 4, FORM, DT>(p, s);
+    default: return launch_tile_instance<OP, 128, 64, 4, 2, 6, 6, FORM, DT>(p, s);
     }
 }
 
