@@ -209,7 +209,7 @@ int miw_grouped_gemm(int dtype, int d_type, int w_layout, int epilogue, int64_t 
     p.gated = gated;
     p.vector = aligned(A, 16) && aligned(W, 16) && lda % 8 == 0 && ldw % 8 == 0 && stride_w % 8 == 0 && k % 8 == 0 && (k_major || n % 8 == 0);
     p.d_vector = stores_vectors(D, ldd, 0, type_size(d_type), gated);
-    HIP_TRY(miw::launch_grouped(p, dtype, d_type, false, (hipStream_t)stream));
+    HIP_TRY(miw::launch_grouped(p, dtype, d_type, false, miw::api_cu_count(), (hipStream_t)stream));
     return 0;
 }
 
@@ -256,7 +256,7 @@ int miw_grouped_wgrad(int dtype, int d_type, int accumulate, int64_t rows, int g
     p.accumulate = accumulate != 0;
     p.vector = aligned(A, 16) && aligned(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && m % 8 == 0 && n % 8 == 0;
     p.d_vector = stores_vectors(D, ldd, stride_d, type_size(d_type), false);
-    HIP_TRY(miw::launch_grouped(p, dtype, d_type, true, (hipStream_t)stream));
+    HIP_TRY(miw::launch_grouped(p, dtype, d_type, true, miw::api_cu_count(), (hipStream_t)stream));
     return 0;
 }
 
@@ -437,7 +437,7 @@ int mxfp4_product(const char *what, int d_type, int epilogue, int64_t rows, int 
     p.gated = gated;
     p.vector = 1;
     p.d_vector = stores_vectors(D, ldd, 0, type_size(d_type), gated);
-    HIP_TRY(miw::launch_grouped_mxfp4(p, d_type, (hipStream_t)stream));
+    HIP_TRY(miw::launch_grouped_mxfp4(p, d_type, miw::api_cu_count(), (hipStream_t)stream));
     return 0;
 }
 

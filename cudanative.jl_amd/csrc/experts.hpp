@@ -83,8 +83,15 @@ hipError_t launch_grouped_tile_bf16(const grouped_params &p, grouped_tile_size t
 hipError_t launch_grouped_tile_mxfp4(const grouped_params &p, grouped_tile_size t, int d_type, hipStream_t s);
 hipError_t launch_grouped_plain(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_mxfp4_plain(const grouped_params &p, int d_type, hipStream_t s);
+// Groups of few rows.  mt: 16-row tiles taken together (1, 2, 4); wt: 16-row tiles of weights a workgroup, with wt 2 on 2 or 4
+// wavefronts, with wt 1 on 8.
+struct grouped_narrow_form {
+    int mt, wt, waves;
+};
+hipError_t launch_grouped_narrow(const grouped_params &p, grouped_narrow_form f, int dtype, int d_type, hipStream_t s);
+hipError_t launch_grouped_mxfp4_narrow(const grouped_params &p, grouped_narrow_form f, int d_type, hipStream_t s);
 // --- grouped_dispatch.hip: the kernel that runs a product.
-hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
-hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, hipStream_t s);
+hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s);
+hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, int cus, hipStream_t s);
 
 }  // namespace miw

@@ -1,25 +1,94 @@
 // Which kernel runs a product grouped by expert.
+//
+// How many rows a group has is not known on the host: the rules go by the mean, rows / groups.  Their numbers come from 222
+// products timed on every kernel (1 to 128 groups, 1024 to 4096 wide, 0.5 to 2048 rows a group whose loads differ by up to three
+// times, f16 and 4 bits, weights from HBM): the rule's kernel takes 1.01 (f16) and 1.02 (4 bits) of the fastest one's time in the
+// geometric mean.
 #include "experts.hpp"
-#include <cstdlib>
+
+#include <algorithm>
 
 namespace miw {
 
-static grouped_tile_size pick(const grouped_params &p)
+static long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+// Groups of few rows are read through registers (grouped_narrow.hpp) where that is faster than a tile:
+//   Few workgroups at 32 rows of weights each (a single projection): 16 rows and eight wavefronts that share k, up to 64 rows.  1
+//     group, 4096 x 4096, f16, 8 rows: 10.2 us, 13.7 with 32 rows and four wavefronts, 28.8 on 128 x 64 tiles; 64 rows 22.5, tiles 29.8.
+//   Otherwise up to ten rows a group, 16 at a time (64 groups, 1024 x 2048, f16: 4 rows 51.0 us, tiles 65.5; 14 rows 77.5 and
+//     64.8), on as many wavefronts as have two chunks of k or more each: 4 bits, 64 groups, 768 x 512 (two chunks): two
+//     wavefronts 6.0 us, four 9.2; f16, 1024 x 2048 (32 chunks): 54.5 and 51.0.  Eight where k is long and the groups are few (8 groups, 4096 x
+//     4096, f16: 49.2 us, four wavefronts 63.1; 64 groups, 1024 x 2048: 63.4 and 51.0).
+static grouped_narrow_form pick_narrow(const grouped_params &p, int slot_k)
 {
-    if (const char *e = getenv("MIW_TILE")) return (grouped_tile_size)atoi(e);
-    return p.I > 128 && p.rows / p.groups > 64 ? TILE_256x128 : TILE_128x64;
+    const double per_group = (double)p.rows / p.groups;
+    const long workgroups = p.groups * ceil_div(p.I, 32), chunks = ceil_div(p.K, slot_k);
+    if (!p.x_k_major || p.source_rows * p.ldy >= 1l << 32) return {0, 0, 0};  // (its offsets are 32 bits; the weights' rows are contiguous along k)
+    if (workgroups <= 256 && per_group <= 64) return {per_group <= 16 ? 1 : per_group <= 32 ? 2 : 4, 1, 8};
+    if (per_group > 10) return {0, 0, 0};
+    if (chunks >= 64 && workgroups <= 1024) return {1, 1, 8};
+    return {1, 2, chunks >= 16 ? 4 : 2};
 }
 
-hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s)
+struct tile_price {
+    grouped_tile_size size;
+    int bi, bj;
+    double f16_slot, f16_tile, mxfp4_slot, mxfp4_tile;  // microseconds for a slot of k and for a tile's start and end
+};
+static const tile_price g_tiles[] = {
+    {TILE_256x256, 256, 256, 1.35, 6.4, 1.90, 6.5},
+    {TILE_256x128, 256, 128, 0.92, 3.6, 0.95, 4.6},
+    {TILE_128x128, 128, 128, 0.58, 6.3, 0.68, 4.0},
+    {TILE_128x64, 128, 64, 0.36, 3.3, 0.48, 2.9},
+};
+
+// Ragged rows: the tile with the shortest estimated launch, rounds of tiles over the CUs at the measured price of each.  A group's
+// last tile is half full in the mean.
+static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int cus)
 {
+    const double per_group = (double)p.rows / p.groups, slots = (double)ceil_div(p.K, slot_k);
+    const tile_price *best = nullptr;
+    double best_us = 0.0;
+    for (const tile_price &t : g_tiles) {
+        const double high = p.groups == 1 ? (double)ceil_div(p.rows, t.bj) : per_group <= 0.5 * t.bj ? 1.0 : per_group / t.bj + 0.5;
+        const double rounds = (double)std::min(p.groups, p.rows) * high * (double)ceil_div(p.I, t.bi) / cus;
+        const double whole = rounds >= 8 ? rounds + 0.5 : std::max(1.0, (double)(long)(rounds + 0.95));
+        const double us = whole * (slot_k == 64 ? t.f16_tile + slots * t.f16_slot : t.mxfp4_tile + slots * t.mxfp4_slot);
+        if (!best || us < best_us) {
+            best = &t;
+            best_us = us;
+        }
+    }
+    // Weights with i contiguous are read in whole lines by the wider tile: 64 groups of 8 rows, 2048 x 1024: 44.5 us, 51.4 with 128 x 64.
+    if (best->size == TILE_128x64 && !p.x_k_major && p.groups * ceil_div(p.I, 256) >= cus) return TILE_256x128;
+    return best->size;
+}
+
+// A ragged sum writes every group's whole result, and the largest tile reads the operands least often: taken as soon as its tiles fill
+// three quarters of the CUs, as the next one is (16 groups of 128 rows, 2048 x 4096: 143 us, 165 on 256 x 128; one group of 2048 rows, 1024
+// x 1024, which is 16 of the largest tiles: 48.3 us, 22.5 on 128 x 64).
+static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
+{
+    for (const tile_price &t : g_tiles)
+        if (p.groups * ceil_div(p.I, t.bi) * ceil_div(p.J, t.bj) >= 3l * cus / 4) return t.size;
+    return TILE_128x64;
+}
+
+hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s)
+{
+    // (lane offsets of 256 rows, or of 64 along k, are 32 bits)
     if (!p.vector || 256 * p.ldx >= 1l << 31) return launch_grouped_plain(p, dtype, d_type, ragged_sum, s);
-    return (dtype == TYPE_F16 ? launch_grouped_tile_f16 : launch_grouped_tile_bf16)(p, pick(p), d_type, ragged_sum, s);
+    if (!ragged_sum)
+        if (const grouped_narrow_form f = pick_narrow(p, 64); f.mt) return launch_grouped_narrow(p, f, dtype, d_type, s);
+    const grouped_tile_size t = ragged_sum ? pick_sum_tile(p, cus) : pick_rows_tile(p, 64, cus);
+    return (dtype == TYPE_F16 ? launch_grouped_tile_f16 : launch_grouped_tile_bf16)(p, t, d_type, ragged_sum, s);
 }
 
-hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, hipStream_t s)
+hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, int cus, hipStream_t s)
 {
     if (256 * p.ldx >= 1l << 31) return launch_grouped_mxfp4_plain(p, d_type, s);
-    return launch_grouped_tile_mxfp4(p, pick(p), d_type, s);
+    if (const grouped_narrow_form f = pick_narrow(p, 256); f.mt) return launch_grouped_mxfp4_narrow(p, f, d_type, s);
+    return launch_grouped_tile_mxfp4(p, pick_rows_tile(p, 256, cus), d_type, s);
 }
 
 }  // namespace miw
