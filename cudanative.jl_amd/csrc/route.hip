@@ -1,14 +1,16 @@
 // Routing of tokens to experts: the choice, its weights, and the order of the rows by expert; the gradient to the logits.
 //
-// Choice.  One wavefront per token, a lane holds logits lane, lane + 64, ...  as unsigned keys in the order of the
-// values (0: never chosen).  The largest key of the wavefront comes from a reduction without LDS, and the lowest expert
-// that has it from one ballot per register, so equal logits go to the lowest expert.
-// Order.  Counting sort: choices are counted per expert and chunk of tokens (integers: no order matters), every chunk
-// then starts at (choices of lower experts) + (choices of this expert in earlier chunks), and one wavefront hands out
-// its chunk's positions in token order.  64 choices at a time find the earlier ones of the same expert by one ballot
-// for each bit of the expert's number.
+// Choice.  A lane holds logits as unsigned keys in the order of the values (0: never chosen).  Up to 256 experts a token has sixteen
+// lanes, four tokens a wavefront: the largest key and the lowest expert that has it are two reductions over a row of lanes by
+// data-parallel moves, so equal logits go to the lowest expert.  What bounds it is the number of instructions: with a wavefront for every
+// token, forty of them a choice in place of fourteen, the first launch of the case below took 12.4 us.  Beyond 256 experts a token has a
+// wavefront, and a ballot per register finds the expert.
+// Order.  Counting sort in two launches over at most 256 chunks of tokens (one launch for up to 64 tokens).  The first counts its chunk's
+// choices of each expert and ranks them: 64 at a time, a wavefront finds the earlier ones of the same expert by one ballot for each
+// bit of the expert's number, and what the 64s before it have is added from a table in LDS.  The second adds up the counts of
+// lower experts and earlier chunks and writes the positions.  Counts are integers: no order of theirs matters.
 //
-// Bound by latency throughout (16 tokens: the launch; 16384 x 128: two launches, and the choice's chain of reductions).
+// Bound by latency throughout: 16381 tokens, 128 experts, 8 choices (bf16): 4.2 MB of logits, MEASURED.
 #include "experts.hpp"
 #include "vec_types.hpp"
 
@@ -16,8 +18,11 @@
 
 namespace miw {
 
-constexpr int ROUTE_THREADS = 512, ROUTE_WAVES = ROUTE_THREADS / 64;
-constexpr int ROUTE_EXPERTS = 1024;
+constexpr int ROUTE_THREADS = 1024, ROUTE_WAVES = ROUTE_THREADS / 64;
+constexpr int ROUTE_EXPERTS = 1024, ROUTE_TOP = 16;
+constexpr int ROUTE_TOKENS = 64;                                      // tokens that a workgroup chooses for at a time
+constexpr int ROUTE_SEGMENTS = ROUTE_TOKENS * ROUTE_TOP / 64;         // of 64 choices
+static_assert(ROUTE_SEGMENTS <= ROUTE_WAVES, "a wavefront for each");
 constexpr float LARGEST = 3.4028234663852886e38f;
 
 // Key of a logit: the order of the keys is that of the values, -0 equals 0, and what is never chosen has key 0.
@@ -32,23 +37,88 @@ __device__ inline float key_value(unsigned key)
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// R: registers that hold a token's logits, ceil(experts / 64).
+// Over the sixteen lanes of a row, to all of them; sums pair the same lanes in every lane.
+template <class F>
+__device__ inline int row_reduce(int v, F join)
+{
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x128 /* row_ror:8 */, 0xf, 0xf, true));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, true));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x122, 0xf, 0xf, true));
+    return join(v, __builtin_amdgcn_update_dpp(0, v, 0x121, 0xf, 0xf, true));
+}
+__device__ inline unsigned row_max(unsigned v) { return (unsigned)row_reduce((int)v, [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); }); }
+__device__ inline int row_min(int v) { return row_reduce(v, [](int a, int b) { return min(a, b); }); }
+__device__ inline float row_sum(float v)
+{
+    return __builtin_bit_cast(float, row_reduce(__builtin_bit_cast(int, v), [](int a, int b) { return __builtin_bit_cast(int, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b)); }));
+}
+
+// Writes choice `lane` of a token (lanes below top), its gate, and the choice into LDS.
+__device__ inline void write_choice(const route_params &p, int base, int token, int lane, int expert, float part, float sum, int *kept)
+{
+    if (lane >= p.top) return;
+    const int at = token * p.top + lane;
+    p.chosen[at] = expert;
+    p.gates[at] = expert >= 0 ? part / sum : 0.f;
+    kept[(token - base) * p.top + lane] = expert;
+}
+
+// Sixteen lanes a token: tokens first .. first + 3, those below last.  R: registers that hold a token's logits, ceil(experts / 16).
+// `kept`: the choices in LDS, those of token `base` first.
 template <class T, int R>
-__device__ inline void choose(const route_params &p, int token, int *hist)
+__device__ inline void choose_row(const route_params &p, int base, int first, int last, int *kept)
+{
+    const int lane = threadIdx.x & 15, token = first + ((threadIdx.x & 63) >> 4);
+    const bool in = token < last;
+    const T *z = (const T *)p.logits + (long)(in ? token : first) * p.ld;
+    unsigned key[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int e = lane + 16 * i;
+        key[i] = e < p.experts ? order_key((float)z[e]) : 0u;
+    }
+    int mine = -1;  // lane j: choice j
+    float value = 0.f, largest = 0.f, every = 0.f;
+    for (int j = 0; j < p.top; j++) {
+        unsigned most = key[0];
+#pragma unroll
+        for (int i = 1; i < R; i++) most = max(most, key[i]);
+        most = row_max(most);
+        int expert = 1 << 30;
+#pragma unroll
+        for (int i = R - 1; i >= 0; i--) expert = key[i] == most ? lane + 16 * i : expert;
+        expert = row_min(expert);
+        const float v = fminf(key_value(most), LARGEST);
+        if (j == 0) {
+            largest = v;
+            if (p.over_all)
+#pragma unroll
+                for (int i = 0; i < R; i++) every += key[i] ? __expf(fminf(key_value(key[i]), LARGEST) - v) : 0.f;
+        }
+        const int hit = (expert & 15) == lane ? expert >> 4 : -1;
+#pragma unroll
+        for (int i = 0; i < R; i++) key[i] = hit == i ? 0u : key[i];
+        if (lane == j && most) {
+            mine = expert;
+            value = v;
+        }
+    }
+    const float part = mine >= 0 ? __expf(value - largest) : 0.f;
+    const float sum = row_sum(p.over_all ? every : part);
+    if (in) write_choice(p, base, token, lane, mine, part, sum, kept);
+}
+
+// A wavefront for the token.  R: ceil(experts / 64).
+template <class T, int R>
+__device__ inline void choose_wave(const route_params &p, int base, int token, int *kept)
 {
     const int lane = threadIdx.x & 63;
     const T *z = (const T *)p.logits + (long)token * p.ld;
     unsigned key[R];
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int e = lane + 64 * i;
-        key[i] = e < p.experts ? order_key((float)z[e]) : 0u;
-    }
-    unsigned all[R];
-#pragma unroll
-    for (int i = 0; i < R; i++) all[i] = key[i];
-    int mine = -1;           // lane j: choice j
-    float value = 0.f, largest = 0.f;
+    for (int i = 0; i < R; i++) key[i] = lane + 64 * i < p.experts ? order_key((float)z[lane + 64 * i]) : 0u;
+    int mine = -1;
+    float value = 0.f, largest = 0.f, every = 0.f;
     for (int j = 0; j < p.top; j++) {
         unsigned most = key[0];
 #pragma unroll
@@ -61,58 +131,23 @@ __device__ inline void choose(const route_params &p, int token, int *hist)
             const unsigned long has = __ballot(key[i] == most);
             if (has) expert = 64 * i + __builtin_ctzl(has);
         }
+        const float v = fminf(key_value(most), LARGEST);
+        if (j == 0) {
+            largest = v;
+            if (p.over_all)
+#pragma unroll
+                for (int i = 0; i < R; i++) every += key[i] ? __expf(fminf(key_value(key[i]), LARGEST) - v) : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < R; i++)
             if (expert == lane + 64 * i) key[i] = 0;
-        const float v = fminf(key_value(most), LARGEST);
-        if (j == 0) largest = v;
         if (lane == j) {
             mine = expert;
             value = v;
         }
     }
     const float part = mine >= 0 ? __expf(value - largest) : 0.f;
-    float sum = part;
-    if (p.over_all) {
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < R; i++)
-            if (all[i]) sum += __expf(fminf(key_value(all[i]), LARGEST) - largest);
-    }
-    sum = wave_sum(sum);
-    if (lane < p.top) {
-        const long at = (long)token * p.top + lane;
-        p.chosen[at] = mine;
-        p.gates[at] = mine >= 0 ? part / sum : 0.f;
-        if (mine >= 0) atomicAdd(&hist[mine], 1);
-    }
-}
-
-// Positions of a chunk's choices.  start: in LDS, the next position of each expert.  One wavefront.
-__device__ inline void place_chunk(const route_params &p, int first, int last, int *start)
-{
-    const int lane = threadIdx.x & 63;
-    for (int at = first * p.top; at < last * p.top; at += 64) {
-        const int i = at + lane;
-        const bool in = i < last * p.top;
-        const int expert = in ? p.chosen[i] : -1;
-        unsigned long same = __ballot(expert >= 0);
-        for (int bit = 0; (p.experts - 1) >> bit; bit++) {
-            const bool set = (expert >> bit) & 1;
-            const unsigned long with = __ballot(set);
-            same &= set ? with : ~with;
-        }
-        const int before = __builtin_popcountl(same & ((1ul << lane) - 1));
-        int position = -1;
-        if (expert >= 0) {
-            position = start[expert] + before;
-            p.rows[position] = i / p.top;
-        }
-        if (in) p.place[i] = position;
-        __builtin_amdgcn_wave_barrier();
-        if (expert >= 0 && (same >> lane) == 1ul) start[expert] = position + 1;  // (the last of them)
-        __builtin_amdgcn_wave_barrier();
-    }
+    write_choice(p, base, token, lane, mine, part, wave_sum(p.over_all ? every : part), kept);
 }
 
 // Turns counts per expert, in LDS, into the first position of each; one wavefront.  Returns the number of choices.
@@ -129,32 +164,79 @@ __device__ inline int first_positions(int experts, int *counts)
     return before;
 }
 
-// WHOLE: one workgroup for all tokens, choice and order in one launch.  A prompt's worth of tokens takes two: the
-// chunks' counts have to be there before any position is known.
-template <class T, int R, bool WHOLE>
+// WHOLE: one workgroup for all tokens, choice and order in one launch.  ROW: sixteen lanes a token, or a wavefront.
+template <class T, int R, bool ROW, bool WHOLE>
 __global__ __launch_bounds__(ROUTE_THREADS) void k_route_choose(route_params p)
 {
-    __shared__ int hist[ROUTE_EXPERTS];
+    __shared__ int kept[ROUTE_TOKENS * ROUTE_TOP];
+    __shared__ unsigned short table[ROUTE_SEGMENTS][ROUTE_EXPERTS];  // choices of each expert in each 64
+    __shared__ int running[ROUTE_EXPERTS];
     __shared__ int total;
-    const int wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) hist[e] = 0;
-    __syncthreads();
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int first = WHOLE ? 0 : blockIdx.x * p.chunk, last = WHOLE ? p.tokens : min(p.tokens, first + p.chunk);
-    for (int t = first + wave; t < last; t += ROUTE_WAVES) choose<T, R>(p, t, hist);
-    __syncthreads();
-    if constexpr (WHOLE) {
-        if (wave == 0) {
-            const int n = first_positions(p.experts, hist);
-            if (threadIdx.x == 0) total = n;
-            __threadfence_block();
-            for (int e = threadIdx.x; e < p.experts; e += 64) p.offsets[e] = hist[e];
-            if (threadIdx.x == 0) p.offsets[p.experts] = n;
-            place_chunk(p, first, last, hist);
+    for (int e = tid; e < p.experts; e += ROUTE_THREADS) running[e] = 0;
+    for (int base = first; base < last; base += ROUTE_TOKENS) {
+        const int end = min(last, base + ROUTE_TOKENS), choices = (end - base) * p.top, segments = (choices + 63) / 64;
+        for (int i = tid; i < segments * p.experts; i += ROUTE_THREADS) table[i / p.experts][i % p.experts] = 0;
+        if constexpr (ROW) {
+            if (base + 4 * wave < end) choose_row<T, R>(p, base, base + 4 * wave, end, kept);
+        } else {
+            for (int t = base + wave; t < end; t += ROUTE_WAVES) choose_wave<T, R>(p, base, t, kept);
         }
         __syncthreads();
-        for (int i = total + (int)threadIdx.x; i < p.tokens * p.top; i += ROUTE_THREADS) p.rows[i] = -1;
+        const int i = wave * 64 + lane;
+        int expert = -1, before = 0;
+        if (wave < segments) {
+            expert = i < choices ? kept[i] : -1;
+            unsigned long same = __ballot(expert >= 0);
+            for (int bit = 0; (p.experts - 1) >> bit; bit++) {
+                const bool set = (expert >> bit) & 1;
+                const unsigned long with = __ballot(set);
+                same &= set ? with : ~with;
+            }
+            before = __builtin_popcountl(same & ((1ul << lane) - 1));
+            if (expert >= 0 && (same >> lane) == 1ul) table[wave][expert] = (unsigned short)(before + 1);  // (the last of them)
+        }
+        __syncthreads();
+        if (i < choices) {
+            int rank = -1;
+            if (expert >= 0) {
+                rank = running[expert] + before;
+                for (int s = 0; s < wave; s++) rank += table[s][expert];
+            }
+            if constexpr (WHOLE) kept[i] = rank;  // (read and written by this thread alone)
+            else p.place[base * p.top + i] = rank;
+        }
+        __syncthreads();
+        for (int e = tid; e < p.experts; e += ROUTE_THREADS) {
+            int sum = running[e];
+            for (int s = 0; s < segments; s++) sum += table[s][e];
+            running[e] = sum;
+        }
+        if constexpr (WHOLE) {
+            __syncthreads();
+            if (wave == 0) {
+                const int n = first_positions(p.experts, running);
+                if (tid == 0) total = n;
+            }
+            __syncthreads();
+            for (int e = tid; e < p.experts; e += ROUTE_THREADS) p.offsets[e] = running[e];
+            if (tid == 0) p.offsets[p.experts] = total;
+            if (i < choices) {
+                const int position = expert >= 0 ? running[expert] + kept[i] : -1;
+                p.place[i] = position;
+                if (position >= 0) p.rows[position] = i / p.top;
+            }
+            for (int at = total + tid; at < p.tokens * p.top; at += ROUTE_THREADS) p.rows[at] = -1;
+        } else {
+            __syncthreads();
+        }
+    }
+    if constexpr (WHOLE) {
+        if (p.tokens == 0)
+            for (int e = tid; e <= p.experts; e += ROUTE_THREADS) p.offsets[e] = 0;
     } else {
-        for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) p.counts[(long)blockIdx.x * p.experts + e] = hist[e];
+        for (int e = tid; e < p.experts; e += ROUTE_THREADS) p.counts[(long)blockIdx.x * p.experts + e] = running[e];
     }
 }
 
@@ -162,119 +244,159 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_place(route_params p)
 {
     __shared__ int counts[ROUTE_EXPERTS], earlier[ROUTE_EXPERTS];
     __shared__ int total;
-    const int wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < p.experts; e += ROUTE_THREADS) counts[e] = earlier[e] = 0;
+    const int tid = threadIdx.x;
+    const int first = blockIdx.x * p.chunk * p.top, last = min(p.tokens, (int)(blockIdx.x + 1) * p.chunk) * p.top;
+    // This thread's first choice is asked for ahead of the counts.
+    int expert = -1, rank = 0;
+    if (first + tid < last) {
+        expert = p.chosen[first + tid];
+        rank = p.place[first + tid];
+    }
+    for (int e = tid; e < p.experts; e += ROUTE_THREADS) counts[e] = earlier[e] = 0;
     __syncthreads();
-    // Several threads add up an expert's chunks where there are fewer experts than threads.
-    const int lanes = ROUTE_THREADS / p.experts < 1 ? 1 : ROUTE_THREADS / p.experts;
-    for (int i = threadIdx.x; i < p.experts * lanes; i += ROUTE_THREADS) {
-        const int e = i % p.experts;
+    // Several threads add up an expert's chunks, eight loads on the way.
+    const int columns = (p.experts + 63) & ~63, slices = ROUTE_THREADS / columns;
+    const int e = tid % columns, slice = tid / columns;
+    if (e < p.experts && slice < slices) {
         int all = 0, before = 0;
-        for (int c = i / p.experts; c < p.chunks; c += lanes) {
-            const int n = p.counts[(long)c * p.experts + e];
-            all += n;
-            if (c < (int)blockIdx.x) before += n;
+        for (int c0 = slice; c0 < p.chunks; c0 += 8 * slices) {
+            int n[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int c = c0 + u * slices;
+                n[u] = c < p.chunks ? p.counts[(long)c * p.experts + e] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                all += n[u];
+                before += c0 + u * slices < (int)blockIdx.x ? n[u] : 0;
+            }
         }
         atomicAdd(&counts[e], all);
         atomicAdd(&earlier[e], before);
     }
     __syncthreads();
-    if (wave == 0) {
+    if (tid < 64) {
         const int n = first_positions(p.experts, counts);
-        if (threadIdx.x == 0) total = n;
-        if (blockIdx.x == 0) {
-            for (int e = threadIdx.x; e < p.experts; e += 64) p.offsets[e] = counts[e];
-            if (threadIdx.x == 0) p.offsets[p.experts] = n;
-        }
-        for (int e = threadIdx.x; e < p.experts; e += 64) earlier[e] += counts[e];
-        __builtin_amdgcn_wave_barrier();
-        const int first = blockIdx.x * p.chunk;
-        place_chunk(p, first, min(p.tokens, first + p.chunk), earlier);
+        if (tid == 0) total = n;
     }
     __syncthreads();
-    for (int i = total + (int)(blockIdx.x * ROUTE_THREADS + threadIdx.x); i < p.tokens * p.top; i += (int)(gridDim.x * ROUTE_THREADS)) p.rows[i] = -1;
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < p.experts; i += ROUTE_THREADS) p.offsets[i] = counts[i];
+        if (tid == 0) p.offsets[p.experts] = total;
+    }
+    for (int at = first + tid; at < last; at += ROUTE_THREADS) {
+        if (at != first + tid) {
+            expert = p.chosen[at];
+            rank = p.place[at];
+        }
+        if (expert < 0) continue;
+        const int position = counts[expert] + earlier[expert] + rank;
+        p.place[at] = position;
+        p.rows[position] = at / p.top;
+    }
+    for (int i = total + (int)(blockIdx.x * ROUTE_THREADS) + tid; i < p.tokens * p.top; i += (int)(gridDim.x * ROUTE_THREADS)) p.rows[i] = -1;
 }
 
-// dz over the chosen: g (dg - sum g dg); over all: p_e (dg_e - sum g dg), dg_e zero where e is not chosen.  A wavefront per token.
-template <class T>
+// dz over the chosen: g (dg - sum g dg); over all: p_e (dg_e - sum g dg), dg_e zero where e is not chosen.  A wavefront per token; its
+// logits, R registers a lane, are asked for together with what it chose.
+template <class T, int R>
 __global__ __launch_bounds__(256) void k_route_grad(route_grad_params p)
 {
     const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (token >= p.tokens) return;
+    const T *z = (const T *)p.logits + (long)token * p.ld;
+    T *dz = (T *)p.dlogits + (long)token * p.ldd;
+    float v[R];
+    if (p.over_all)
+#pragma unroll
+        for (int i = 0; i < R; i++) v[i] = lane + 64 * i < p.experts ? (float)z[lane + 64 * i] : -__builtin_inff();
     const long at = (long)token * p.top + lane;
     int expert = -1;
     float gate = 0.f, dgate = 0.f;
     if (lane < p.top) {
         expert = p.chosen[at];
         gate = p.gates[at];
-        if (expert >= 0) dgate = p.dgates[at];  // (what a choice without an expert gets is not looked at)
+        dgate = p.dgates[at];
     }
+    if (expert < 0) gate = dgate = 0.f;  // (what a choice without an expert gets is not looked at)
     const float inner = wave_sum(gate * dgate);
-    const T *z = (const T *)p.logits + (long)token * p.ld;
-    T *dz = (T *)p.dlogits + (long)token * p.ldd;
-    // The softmax over all logits from its largest: choice 0 is the largest logit.
-    const int first = __builtin_amdgcn_readlane(expert, 0);
-    const bool all = p.over_all && first >= 0 && first < p.experts;
-    float largest = 0.f, total = 1.f;
-    if (all) {
-        largest = fminf((float)z[first], LARGEST);
+    const float direct = p.over_all ? gate * dgate : gate * (dgate - inner);
+    float total = 1.f;
+    if (p.over_all) {
+        // The softmax over all logits from its largest.
+        unsigned most = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++) most = max(most, order_key(v[i]));
+        most = wave_max(most);
+        const float largest = most ? fminf(key_value(most), LARGEST) : 0.f;
         float sum = 0.f;
-        for (int e = lane; e < p.experts; e += 64) {
-            const float v = (float)z[e];
-            if (v > -__builtin_inff()) sum += __expf(fminf(v, LARGEST) - largest);
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            v[i] = v[i] > -__builtin_inff() ? __expf(fminf(v[i], LARGEST) - largest) : 0.f;  // (NaN: 0)
+            sum += v[i];
         }
         total = wave_sum(sum);
+        if (total == 0.f) total = 1.f;
     }
-    for (int e0 = 0; e0 < p.experts; e0 += 64) {
-        const int e = e0 + lane;
-        float own = 0.f;
-        bool chosen = false;
-        for (int j = 0; j < p.top; j++) {
-            const int x = __builtin_amdgcn_readlane(expert, j);
-            const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p.over_all ? gate * dgate : gate * (dgate - inner)), j));
-            if (x == e) {
-                own = v;
-                chosen = true;
-            }
-        }
-        if (e >= p.experts) continue;
-        float d = chosen ? own : 0.f;
-        if (all) {
-            const float v = (float)z[e];
-            if (v > -__builtin_inff()) d -= __expf(fminf(v, LARGEST) - largest) / total * inner;
-        }
-        dz[e] = (T)d;
+    float d[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) d[i] = p.over_all ? -(v[i] / total) * inner : 0.f;
+    for (int j = 0; j < p.top; j++) {
+        const int x = __builtin_amdgcn_readlane(expert, j);
+        const float add = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, direct), j));
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (x == lane + 64 * i) d[i] += add;
     }
+#pragma unroll
+    for (int i = 0; i < R; i++)
+        if (lane + 64 * i < p.experts) dz[lane + 64 * i] = (T)d[i];
 }
 
-// One workgroup as long as its wavefronts have no more than eight tokens each and its one placing wavefront sixteen rounds.
-int route_chunks(long tokens, int top)
+// At most 256 chunks of sixteen tokens (one a wavefront) or more; one workgroup as long as it has its tokens together.
+static int route_chunk(long tokens)
 {
-    if (tokens <= 8 * ROUTE_WAVES && tokens * top <= 1024) return 1;
-    const long chunk = (tokens + 255) / 256 > ROUTE_WAVES ? (tokens + 255) / 256 : ROUTE_WAVES;
-    return (int)((tokens + chunk - 1) / chunk);
+    const long chunk = (tokens + 255) / 256;
+    return (int)(chunk < ROUTE_WAVES ? ROUTE_WAVES : chunk);
+}
+int route_chunks(long tokens)
+{
+    return tokens <= ROUTE_TOKENS ? 1 : (int)((tokens + route_chunk(tokens) - 1) / route_chunk(tokens));
+}
+
+template <class F>
+static void with_registers(int experts, F go)
+{
+    const int r = (experts + 63) / 64;
+    if (r == 1) go(std::integral_constant<int, 1>{});
+    else if (r == 2) go(std::integral_constant<int, 2>{});
+    else if (r <= 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 16>{});
+}
+template <class F>
+static void with_type(int dtype, F go)
+{
+    if (dtype == TYPE_F32) go(float{});
+    else if (dtype == TYPE_F16) go(f16_t{});
+    else go(bf16_t{});
 }
 
 hipError_t launch_route(route_params p, int dtype, hipStream_t s)
 {
-    p.chunks = route_chunks(p.tokens, p.top);
-    p.chunk = (p.tokens + p.chunks - 1) / p.chunks;
-    const int r = (p.experts + 63) / 64;
-    auto go = [&](auto type, auto regs) {
+    p.chunks = route_chunks(p.tokens);
+    p.chunk = route_chunk(p.tokens);
+    with_type(dtype, [&](auto type) {
         using T = decltype(type);
-        constexpr int R = decltype(regs)::value;
-        if (p.chunks == 1) hipLaunchKernelGGL((k_route_choose<T, R, true>), dim3(1), dim3(ROUTE_THREADS), 0, s, p);
-        else hipLaunchKernelGGL((k_route_choose<T, R, false>), dim3((unsigned)p.chunks), dim3(ROUTE_THREADS), 0, s, p);
-    };
-    auto typed = [&](auto type) {
-        if (r == 1) go(type, std::integral_constant<int, 1>{});
-        else if (r == 2) go(type, std::integral_constant<int, 2>{});
-        else if (r <= 4) go(type, std::integral_constant<int, 4>{});
-        else go(type, std::integral_constant<int, 16>{});
-    };
-    if (dtype == TYPE_F32) typed(float{});
-    else if (dtype == TYPE_F16) typed(f16_t{});
-    else typed(bf16_t{});
+        auto go = [&](auto regs, auto row) {
+            constexpr int R = decltype(regs)::value;
+            constexpr bool ROW = decltype(row)::value;
+            if (p.chunks == 1) hipLaunchKernelGGL((k_route_choose<T, R, ROW, true>), dim3(1), dim3(ROUTE_THREADS), 0, s, p);
+            else hipLaunchKernelGGL((k_route_choose<T, R, ROW, false>), dim3((unsigned)p.chunks), dim3(ROUTE_THREADS), 0, s, p);
+        };
+        if (p.experts > 256) go(std::integral_constant<int, 16>{}, std::false_type{});
+        else with_registers(p.experts, [&](auto regs) { go(std::integral_constant<int, 4 * decltype(regs)::value>{}, std::true_type{}); });
+    });
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.chunks == 1) return e;
     hipLaunchKernelGGL(k_route_place, dim3((unsigned)p.chunks), dim3(ROUTE_THREADS), 0, s, p);
@@ -284,9 +406,11 @@ hipError_t launch_route(route_params p, int dtype, hipStream_t s)
 hipError_t launch_route_grad(const route_grad_params &p, int dtype, hipStream_t s)
 {
     const dim3 grid((unsigned)((p.tokens + 3) / 4)), block(256);
-    if (dtype == TYPE_F32) hipLaunchKernelGGL(k_route_grad<float>, grid, block, 0, s, p);
-    else if (dtype == TYPE_F16) hipLaunchKernelGGL(k_route_grad<f16_t>, grid, block, 0, s, p);
-    else hipLaunchKernelGGL(k_route_grad<bf16_t>, grid, block, 0, s, p);
+    with_type(dtype, [&](auto type) {
+        with_registers(p.experts, [&](auto regs) {
+            hipLaunchKernelGGL((k_route_grad<decltype(type), decltype(regs)::value>), grid, block, 0, s, p);
+        });
+    });
     return hipGetLastError();
 }
 
