@@ -76,13 +76,14 @@ struct grouped_params {
     int gated, accumulate;
     int vector;   // 16-byte accesses to the operands
     int d_vector; // aligned stores of four elements
+    int most_tiles;  // workgroups that the tiles need, one each, rounded up to whole eighths; set by the launch
 };
 enum grouped_tile_size { TILE_256x256, TILE_256x128, TILE_128x128, TILE_128x64 };
 hipError_t launch_grouped_tile_f16(const grouped_params &p, grouped_tile_size t, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_tile_bf16(const grouped_params &p, grouped_tile_size t, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_tile_mxfp4(const grouped_params &p, grouped_tile_size t, int d_type, hipStream_t s);
-hipError_t launch_grouped_plain(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
-hipError_t launch_grouped_mxfp4_plain(const grouped_params &p, int d_type, hipStream_t s);
+hipError_t launch_grouped_plain(grouped_params p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
+hipError_t launch_grouped_mxfp4_plain(grouped_params p, int d_type, hipStream_t s);
 // Groups of few rows.  mt: 16-row tiles taken together (1, 2, 4); wt: 16-row tiles of weights a workgroup, with wt 2 on 2 or 4
 // wavefronts, with wt 1 on 8.
 struct grouped_narrow_form {

@@ -10,14 +10,16 @@ namespace miw {
 struct group_rows {
     int first, last;
 };
-__device__ inline group_rows rows_of_group(const grouped_params &p, int g)
+template <class PARAMS>
+__device__ inline group_rows rows_of_group(const PARAMS &p, int g)
 {
     if (!p.offsets) return {0, p.rows};
     const int first = min(max(p.offsets[g], 0), p.rows), last = min(max(p.offsets[g + 1], 0), p.rows);
     return {first, max(first, last)};
 }
 // Row of the gathered operand at a sorted position.
-__device__ inline int source_row(const grouped_params &p, int position)
+template <class PARAMS>
+__device__ inline int source_row(const PARAMS &p, int position)
 {
     const int row = p.gather ? p.gather[position] : position;
     return min(max(row, 0), p.source_rows - 1);
@@ -32,9 +34,9 @@ constexpr int GROUP_J_TILES = 8;
 // Workgroup -> tile, or -1.  Workgroups go round-robin over the eight XCDs; 256 tiles at a time are cut into eight runs.  (One run
 // of all tiles for each XCD gives it whole groups, and the XCD with the longest ones ends last: the gradient to the
 // weights of 16 uneven groups, 4096 x 2048 each, took 314 us like that.)
-__device__ inline int tile_of_workgroup(int total)
+__device__ inline int tile_of_workgroup(int total, int workgroup)
 {
-    const int xcd = (int)blockIdx.x & 7, loc = (int)blockIdx.x >> 3;
+    const int xcd = workgroup & 7, loc = workgroup >> 3;
     const int whole = total >> 8, rest = total & 255;
     if (loc < whole * 32) return (loc >> 5) * 256 + xcd * 32 + (loc & 31);
     const int run = (rest + 7) >> 3, at = loc - whole * 32, tile = xcd * run + at;
@@ -43,7 +45,8 @@ __device__ inline int tile_of_workgroup(int total)
 struct grouped_tile {
     int group, first, last, j0, i0;  // first, last: the group's rows; j0: first row of the tile; group -1: no tile
 };
-__device__ inline grouped_tile find_tile(const grouped_params &p, int bi, int bj)
+template <class PARAMS>
+__device__ inline grouped_tile find_tile(const PARAMS &p, int bi, int bj, int workgroup)
 {
     const int lane = (int)threadIdx.x & 63;
     const int tiles_i = (p.I + bi - 1) / bi;
@@ -55,8 +58,8 @@ __device__ inline grouped_tile find_tile(const grouped_params &p, int bi, int bj
     int c = count(lane), upto = wave_scan(c);
     int total = __builtin_amdgcn_readlane(upto, 63);
     for (int g0 = 64; g0 < p.groups; g0 += 64) total += __builtin_amdgcn_readlane(wave_scan(count(g0 + lane)), 63);
-    total = min(max(total, 0) * tiles_i, (int)gridDim.x);
-    int id = tile_of_workgroup(total);
+    total = min(max(total, 0) * tiles_i, p.most_tiles);
+    int id = tile_of_workgroup(total, workgroup);
     if (id < 0) return {-1, 0, 0, 0, 0};
     const int row_tile = id / tiles_i;  // (of all groups; a group's tiles are numbered together)
     int g0 = 0, before = 0;
@@ -94,8 +97,8 @@ __device__ inline float gated_silu(float gate, float value) { return gate / (1.f
 
 // Stores the four results i .. i + 3 of row j; those from I on are left out.  In the gated form they are two pairs of gate and
 // value, and two results are stored (I counts the columns before that).
-template <class DT>
-__device__ inline void store_results(const grouped_params &p, DT *row, int i, f32x4 v)
+template <class DT, class PARAMS>
+__device__ inline void store_results(const PARAMS &p, DT *row, int i, f32x4 v)
 {
     if (i >= p.I) return;
     if (p.gated) {

@@ -76,8 +76,8 @@ static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
 
 hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s)
 {
-    // (lane offsets of 256 rows, or of 64 along k, are 32 bits)
-    if (!p.vector || 256 * p.ldx >= 1l << 31) return launch_grouped_plain(p, dtype, d_type, ragged_sum, s);
+    // (lane offsets of 256 rows, or of 64 along k, are 32 bits; a sum over no rows has none to fetch)
+    if (!p.vector || 256 * p.ldx >= 1l << 31 || p.rows == 0) return launch_grouped_plain(p, dtype, d_type, ragged_sum, s);
     if (!ragged_sum)
         if (const grouped_narrow_form f = pick_narrow(p, 64); f.mt) return launch_grouped_narrow(p, f, dtype, d_type, s);
     const grouped_tile_size t = ragged_sum ? pick_sum_tile(p, cus) : pick_rows_tile(p, 64, cus);

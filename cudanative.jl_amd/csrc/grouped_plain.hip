@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void k_grouped_plain(grouped_params p)
         length = range.last - range.first;
         if (length == 0 && p.accumulate) return;
     } else {
-        const grouped_tile t = find_tile(p, PLAIN, PLAIN);
+        const grouped_tile t = find_tile(p, PLAIN, PLAIN, (int)blockIdx.x);
         if (t.group < 0) return;
         group = t.group;
         i0 = t.i0;
@@ -94,10 +94,11 @@ __global__ __launch_bounds__(256) void k_grouped_plain(grouped_params p)
     }
 }
 
-hipError_t launch_grouped_plain(const grouped_params &p, int dtype, int d_type, bool ragged_sum, hipStream_t s)
+hipError_t launch_grouped_plain(grouped_params p, int dtype, int d_type, bool ragged_sum, hipStream_t s)
 {
     const long blocks = ragged_sum ? (long)p.groups * ((p.I + PLAIN - 1) / PLAIN) * ((p.J + PLAIN - 1) / PLAIN) : grouped_blocks(p, PLAIN, PLAIN, 256);
     if (blocks <= 0 || blocks >= 1l << 24) return hipErrorInvalidConfiguration;
+    p.most_tiles = (int)blocks;
     const dim3 grid((unsigned)blocks), block(256);
     auto go = [&](auto mfma, auto type) {
         using M = decltype(mfma);
@@ -116,7 +117,7 @@ hipError_t launch_grouped_plain(const grouped_params &p, int dtype, int d_type, 
 template <class DT>
 __global__ __launch_bounds__(64) void k_grouped_mxfp4_plain(grouped_params p)
 {
-    const grouped_tile t = find_tile(p, 16, 16);
+    const grouped_tile t = find_tile(p, 16, 16, (int)blockIdx.x);
     if (t.group < 0) return;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     const int i = min(t.i0 + r, p.I - 1), j = source_row(p, min(t.j0 + r, t.last - 1));
@@ -139,10 +140,11 @@ __global__ __launch_bounds__(64) void k_grouped_mxfp4_plain(grouped_params p)
     if (t.j0 + r < t.last) store_results<DT>(p, (DT *)p.D + (long)(t.j0 + r) * p.ldd, t.i0 + 4 * q, acc);
 }
 
-hipError_t launch_grouped_mxfp4_plain(const grouped_params &p, int d_type, hipStream_t s)
+hipError_t launch_grouped_mxfp4_plain(grouped_params p, int d_type, hipStream_t s)
 {
     const long blocks = grouped_blocks(p, 16, 16, 64);
     if (blocks <= 0) return hipErrorInvalidConfiguration;
+    p.most_tiles = (int)blocks;
     const dim3 grid((unsigned)blocks), block(64);
     if (d_type == TYPE_F32) hipLaunchKernelGGL(k_grouped_mxfp4_plain<float>, grid, block, 0, s, p);
     else if (d_type == TYPE_F16) hipLaunchKernelGGL(k_grouped_mxfp4_plain<f16_t>, grid, block, 0, s, p);

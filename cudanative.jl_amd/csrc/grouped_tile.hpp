@@ -51,11 +51,20 @@ constexpr int grouped_lds_bytes(int bi, int bj, int nx, int ny, bool scaled, int
     return nx * grouped_slot_bytes(bi, scaled) + ny * grouped_slot_bytes(bj, scaled) + (form == RAGGED_SUM ? 2 * ny * 256 : 0);
 }
 
+// Workgroups that a CU holds together.
+constexpr int grouped_workgroups(int bi, int bj, int nx, int ny, bool scaled, int form)
+{
+    return grouped_lds_bytes(bi, bj, nx, ny, scaled, form) <= 80 * 1024 ? 2 : 1;
+}
+// Do workgroups walk several tiles?
+constexpr bool grouped_walks(bool scaled, int form) { return !scaled && form != RAGGED_SUM; }
+
 // Tile of a ragged sum: groups one after the other, eight tiles along j together.
-__device__ inline grouped_tile find_sum_tile(const grouped_params &p, int bi, int bj)
+template <class PARAMS>
+__device__ inline grouped_tile find_sum_tile(const PARAMS &p, int bi, int bj, int workgroup)
 {
     const int tiles_i = (p.I + bi - 1) / bi, tiles_j = (p.J + bj - 1) / bj;
-    int id = tile_of_workgroup(p.groups * tiles_i * tiles_j);
+    int id = tile_of_workgroup(p.groups * tiles_i * tiles_j, workgroup);
     if (id < 0) return {-1, 0, 0, 0, 0};
     const int group = id / (tiles_i * tiles_j);
     id -= group * tiles_i * tiles_j;
@@ -80,7 +89,7 @@ __device__ inline void keep_first(u32x4 &f, int keep)
 //     has to have landed at the end of the second; X's goes with it, or, with three slots of X, the one after that in the
 //     second cluster, so that X, the weights, which come from HBM where the rows mostly come from caches, has twice the time.
 template <class OP, int BI, int BJ, int WI, int WJ, int NX, int NY, int FORM, class DT>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * grouped_workgroups(BI, BJ, NX, NY, OP::scaled, FORM))))
 void k_grouped_tile(grouped_params p)
 {
     constexpr int NT = 512;
@@ -102,81 +111,96 @@ void k_grouped_tile(grouped_params p)
 
     extern __shared__ __attribute__((aligned(128))) char smem[];
     MIW_LDS char *lds = (MIW_LDS char *)smem;
-    const grouped_tile at = SUM ? find_sum_tile(p, BI, BJ) : find_tile(p, BI, BJ);
-    if (at.group < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave % WI, wj = wave / WI, q = lane >> 4, r = lane & 15;
     const bool late_group = wave >= 4;
-    const int length = SUM ? at.last - at.first : p.K;  // of the sum
-    const int NP = (length + OP::slot_k - 1) / OP::slot_k;
-    if (SUM && NP == 0 && p.accumulate) return;
-
-    // This thread's chunk of a load: row (k) tid / 8, and the 16 bytes of it that go to place tid % 8.
-    const int line = tid >> 3, place = tid & 7;
-    const int k_chunk = place ^ ((line >> 1) & 7), i_chunk = place ^ (2 * i_major_swizzle(line));
-    // Chunks of 16 bytes (8 values of k) that the last slot has: all lanes fetch valid ones.
-    const int last_values = length - (NP - 1) * OP::slot_k;
-    const int last_chunks = SCALED ? (last_values + 31) / 32 : (last_values + 7) / 8;
-
-    const char *X = p.X + (SUM ? 0 : (long)at.group * p.sx);
-    const char *Y = p.Y;
-    // X: a uniform origin that moves with the slots and a lane offset for each load.
-    unsigned xvo[NLX];
-    const char *yp[NLY];
-    if constexpr (XK) {
-        X += (long)at.i0 * p.ldx;
-#pragma unroll
-        for (int i = 0; i < NLX; i++) xvo[i] = (unsigned)(min(line + 64 * i, p.I - 1 - at.i0) * (int)p.ldx + k_chunk * 16);
-    } else {
-        X += 2l * at.i0;
-#pragma unroll
-        for (int i = 0; i < NLX; i++) xvo[i] = (SUM ? 0u : (unsigned)(line * (int)p.ldx)) + 2u * (unsigned)min(64 * i + i_chunk * 8, p.I - 8 - at.i0);
-    }
-    if constexpr (YK) {
-#pragma unroll
-        for (int i = 0; i < NLY; i++) yp[i] = Y + (long)source_row(p, min(at.j0 + line + 64 * i, at.last - 1)) * p.ldy + k_chunk * 16;
-    } else {
-#pragma unroll
-        for (int i = 0; i < NLY; i++) yp[i] = Y + 2l * (at.j0 + min(64 * i + i_chunk * 8, p.J - 8 - at.j0));
-    }
+    const int line = tid >> 3;  // this thread's row (k) of a load
+    // Between tiles the arguments are read again and what hangs on the thread's number is made again: kept through the K loop
+    // they would take more registers than there are.
+    auto arguments = [] MIW_INLINE {
+        auto a = (const __attribute__((address_space(4))) grouped_params *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
+    };
+    auto thread = [] MIW_INLINE {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        return t;
+    };
+    // The 16 bytes of a load's row that go to place t % 8 of it, where k is contiguous and where i is.
+    auto k_chunk_of = [](int t) MIW_INLINE { return (t & 7) ^ ((t >> 4) & 7); };
+    auto i_chunk_of = [](int t) MIW_INLINE { return (t & 7) ^ (2 * i_major_swizzle(t >> 3)); };
     // Scales: X's are fetched 16 bytes (two rows) a lane, Y's, whose rows may lie anywhere, four bytes a lane.  Where the
     // wavefronts suffice the first ones fetch X's and the others Y's, one load each; otherwise every one fetches a part of
     // both.  All count the same: those that are left over repeat another's.
     static_assert(!SCALED || (XSW <= 8 && YSW <= 8), "loads of scales");
     const bool x_scales = SHARED_SCALES && wave < XSW;
     const int x_part = wave % XSW, y_part = SHARED_SCALES ? (wave + YSW - XSW % YSW) % YSW : wave % YSW;
-    const char *xsp = nullptr, *ysp = nullptr;
-    if constexpr (SCALED) {
-        xsp = (const char *)p.xs + (long)at.group * p.sxs + 8l * min((long)at.i0 + x_part * 128 + 2 * lane, p.lxs - 2);
-        const int dword = y_part * 64 + lane;
-        ysp = (const char *)p.ys + 8l * source_row(p, min(at.j0 + (dword >> 1), at.last - 1)) + 4 * (dword & 1);
-    }
-    const long x_step = XK ? 128 : 64 * p.ldx;
 
+    // A workgroup walks tiles.  Which one is next, and the rows that its first requests need, is looked up while the first slots of
+    // the one before are on the way, and these are requested ahead of the stores of the one before that: what is left
+    // of a tile's start is the wait for its first slot.
+    constexpr int ROWS = YK ? NLY : NY - 1;
+    struct walked_tile {
+        grouped_tile at;
+        int rows[ROWS];  // ragged rows: of this thread's lines of Y; ragged sum: of its line of the first slots of X
+        int scale_row;
+    };
+    auto find = [&](int workgroup) MIW_INLINE {
+        walked_tile t;
+        const auto a = arguments();
+        const int me = thread(), line = me >> 3;
+        grouped_tile at;
+        if constexpr (SUM) at = find_sum_tile(*a, BI, BJ, workgroup);
+        else at = find_tile(*a, BI, BJ, workgroup);
+        t.at = {__builtin_amdgcn_readfirstlane(at.group), __builtin_amdgcn_readfirstlane(at.first), __builtin_amdgcn_readfirstlane(at.last),
+                __builtin_amdgcn_readfirstlane(at.j0), __builtin_amdgcn_readfirstlane(at.i0)};
+        t.scale_row = 0;
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) t.rows[i] = 0;
+        if (t.at.group >= 0 && t.at.first < t.at.last) {
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) t.rows[i] = source_row(*a, min((YK ? t.at.j0 : t.at.first) + line + 64 * i, t.at.last - 1));
+            if constexpr (SCALED) t.scale_row = source_row(*a, min(t.at.j0 + 32 * y_part + ((me & 63) >> 1), t.at.last - 1));
+        }
+        return t;
+    };
+    int workgroup = (int)blockIdx.x;
+    walked_tile tile = find(workgroup);
+    if (tile.at.group < 0) return;
+    grouped_tile at = tile.at;
+
+    int length, NP, last_values, last_chunks;  // of the sum, in values and slots; values and 16-byte chunks that its last slot has
+    const char *X;           // a uniform origin that moves with the slots, and a lane offset for each load
+    unsigned xvo[NLX];
+    const char *yp[NLY];
+    const char *xsp = nullptr, *ysp = nullptr;
+    const long x_step = XK ? 128 : 64 * p.ldx;
     const unsigned wave_dst = (unsigned)(uintptr_t)lds + (unsigned)wave * 1024u;
     const unsigned lds0 = (unsigned)(uintptr_t)lds;
-    int xnext = 0, ynext = 0;    // slots to request (one number, ynext, without SPLIT)
-    unsigned xwoff = 0, ywoff = 0;  // their places in the rings
+    int xnext, ynext;       // slots to request (one number, ynext, without SPLIT)
+    unsigned xwoff, ywoff;  // their places in the rings
     long xrow = 0, yrow = 0;     // (ragged sum: the lane's rows of the slot, in bytes from the operands)
     auto x_last_begins = [&]() MIW_INLINE {
         if constexpr (SUM) return;
+        const int me = thread(), line = me >> 3, k_chunk = k_chunk_of(me);
         const unsigned back = XK ? 16u * (unsigned)max(0, k_chunk - (last_chunks - 1)) : (unsigned)(max(0, line - (last_values - 1)) * (int)p.ldx);
 #pragma unroll
         for (int i = 0; i < NLX; i++) xvo[i] -= back;
     };
     auto y_last_begins = [&]() MIW_INLINE {
         if constexpr (SUM) return;
+        const int k_chunk = k_chunk_of(thread());
         const int back = 16 * max(0, k_chunk - (last_chunks - 1));
 #pragma unroll
         for (int i = 0; i < NLY; i++) yp[i] -= back;
     };
     // Ragged sum: where this lane's row of slot `ynext` lies in both operands.
     auto find_rows = [&](int gathered) MIW_INLINE {
-        const int position = min(at.first + ynext * 64 + line, at.last - 1);
+        const int position = max(min(at.first + ynext * 64 + line, at.last - 1), 0);
         yrow = (long)position * p.ldy;
         xrow = (long)gathered * p.ldx;
     };
-    auto direct_row = [&]() MIW_INLINE { return source_row(p, min(at.first + ynext * 64 + line, at.last - 1)); };
     auto index_entry = [&](int slot) MIW_INLINE { return (unsigned)(slot % (2 * NY)) * 256u; };
     // Load N of a slot: X's, Y's, then what goes with them.
     auto request_one = [&]<int N>(std::integral_constant<int, N>) MIW_INLINE {
@@ -195,7 +219,7 @@ void k_grouped_tile(grouped_params p)
             else lds_load4<XRING + YBYTES>(ysp, lds0 + ywoff + (unsigned)y_part * 256u);
         } else if constexpr (SUM) {
             // the rows of the slot NY - 1 further on, by every wavefront to the same place
-            const int position = min(at.first + min(ynext + NY - 1, NP - 1) * 64 + lane, at.last - 1);
+            const int position = max(min(at.first + min(ynext + NY - 1, NP - 1) * 64 + lane, at.last - 1), 0);
             lds_load4<INDEX>((const char *)(p.gather ? p.gather + position : p.offsets), lds0 + index_entry(ynext + NY - 1));
         }
     };
@@ -226,28 +250,47 @@ void k_grouped_tile(grouped_params p)
         }
     };
 
-    frag_reader<BI, XK> xr;
-    frag_reader<BJ, YK> yr;
-    xr.init(wi * WTI, lane);
-    yr.init(wj * WTJ, lane);
-    f32x4 acc[TI][TJ];
+    // Turns to a tile and requests its first slots (a sum that is shorter than the rings asks for its last slot again, which
+    // nobody reads, and one of no rows for the row before).  The rings are empty then, and start at their beginnings.
+    auto start = [&](const walked_tile &t) MIW_INLINE {
+        const auto a = arguments();
+        const int me = thread(), line = me >> 3, k_chunk = k_chunk_of(me), i_chunk = i_chunk_of(me);
+        at = t.at;
+        length = SUM ? at.last - at.first : a->K;
+        NP = (length + OP::slot_k - 1) / OP::slot_k;
+        last_values = length - (NP - 1) * OP::slot_k;
+        last_chunks = SCALED ? (last_values + 31) / 32 : (last_values + 7) / 8;
+        xnext = ynext = 0;
+        xwoff = ywoff = 0;
+        X = a->X + (SUM ? 0 : (long)at.group * a->sx);
+        if constexpr (XK) {
+            X += (long)at.i0 * a->ldx;
 #pragma unroll
-    for (int a = 0; a < TI; a++)
+            for (int i = 0; i < NLX; i++) xvo[i] = (unsigned)(min(line + 64 * i, a->I - 1 - at.i0) * (int)a->ldx + k_chunk * 16);
+        } else {
+            X += 2l * at.i0;
 #pragma unroll
-        for (int b = 0; b < TJ; b++) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (NP > 0) {
+            for (int i = 0; i < NLX; i++) xvo[i] = (SUM ? 0u : (unsigned)(line * (int)a->ldx)) + 2u * (unsigned)min(64 * i + i_chunk * 8, a->I - 8 - at.i0);
+        }
+#pragma unroll
+        for (int i = 0; i < NLY; i++) {
+            if constexpr (YK) yp[i] = a->Y + (long)t.rows[i] * a->ldy + k_chunk * 16;
+            else yp[i] = a->Y + 2l * (at.j0 + min(64 * i + i_chunk * 8, a->J - 8 - at.j0));
+        }
+        if constexpr (SCALED) {
+            xsp = (const char *)a->xs + (long)at.group * a->sxs + 8l * min((long)at.i0 + x_part * 128 + 2 * (me & 63), a->lxs - 2);
+            ysp = (const char *)a->ys + 8l * t.scale_row + 4 * (me & 1);
+        }
         if (NP == 1) {
             x_last_begins();
             y_last_begins();
         }
-        // The first slots (a sum that is shorter than the rings asks for its last slot again, which nobody reads).
         constexpr std::integral_constant<int, 0> first_load{};
         constexpr std::integral_constant<int, NLX> x_loads{};
         constexpr std::integral_constant<int, LPAIR> all_loads{};
 #pragma unroll
         for (int s = 0; s < NY - 1; s++) {
-            if constexpr (SUM) find_rows(direct_row());
+            if constexpr (SUM) find_rows(t.rows[s]);
             request_all(first_load, all_loads);
             x_end_request();
             y_end_request();
@@ -255,11 +298,63 @@ void k_grouped_tile(grouped_params p)
         if constexpr (SPLIT) {
             request_all(first_load, x_loads);
             x_end_request();
-            wait_loads_and_barrier<NLX>();
-        } else {
-            wait_loads_and_barrier<(NY - 2) * LPAIR>();
         }
+    };
 
+    frag_reader<BI, XK> xr;
+    frag_reader<BJ, YK> yr;
+    xr.init(wi * WTI, lane);
+    yr.init(wj * WTJ, lane);
+    f32x4 acc[TI][TJ];
+
+    // Neighbouring lanes hold neighbouring rows: they exchange the results of two MFMA tiles, so that a row's 32 go out together
+    // (128 bytes of Float32) from eight lanes, first the even rows and then the odd ones.  Whole tiles are stored by TI * TJ
+    // instructions of each wavefront; true is returned then.
+    auto store_tile = [&](const grouped_tile &t) MIW_INLINE {
+        const auto args = arguments();
+        const int me = thread(), q = (me & 63) >> 4, r = me & 15;
+        if (SUM && args->accumulate && t.first >= t.last) return false;
+        DT *D = (DT *)args->D + (SUM ? (long)t.group * args->sd : 0);
+        const int end_j = SUM ? args->J : t.last;
+        const bool odd = r & 1;
+        const bool whole = args->d_vector && !args->gated && !args->accumulate && t.i0 + BI <= args->I && t.j0 + BJ <= end_j;
+#pragma unroll
+        for (int b = 0; b < TJ; b++) {
+            const int j = t.j0 + wj * WTJ + 16 * b + (r & ~1);
+            DT *row = D + (long)j * args->ldd;
+#pragma unroll
+            for (int a = 0; a < TI; a += 2) {
+                float4_t v0 = acc[a][b], v1 = acc[a + 1][b];
+                pair_exchange(odd, v0, v1);
+                const int i = t.i0 + wi * WTI + 16 * (a + odd) + 4 * q;
+                __builtin_amdgcn_sched_barrier(0);  // (two tiles' registers at a time)
+                if (whole) {
+                    *(vec<DT, 4> *)(row + i) = __builtin_convertvector(v0, vec<DT, 4>);
+                    *(vec<DT, 4> *)(row + args->ldd + i) = __builtin_convertvector(v1, vec<DT, 4>);
+                } else {
+                    if (j < end_j) store_results<DT>(*args, row, i, v0);
+                    if (j + 1 < end_j) store_results<DT>(*args, row + args->ldd, i, v1);
+                }
+            }
+        }
+        return whole;
+    };
+
+    constexpr bool WALKS = grouped_walks(SCALED, FORM);
+    start(tile);
+    if constexpr (WALKS) {
+        workgroup += (int)gridDim.x;
+        tile = find(workgroup);
+    }
+    wait_loads_and_barrier<0>();
+    for (;;) {
+    float zero = 0.f;
+    asm volatile("" : "+s"(zero));  // (otherwise a zero vector is kept in registers through the tiles)
+#pragma unroll
+    for (int a = 0; a < TI; a++)
+#pragma unroll
+        for (int b = 0; b < TJ; b++) acc[a][b] = f32x4{zero, zero, zero, zero};
+    if (NP > 0) {
         constexpr int FSETS = HALVES ? 1 : 2;
         u32x4 fx[FSETS][TI], fy[FSETS][TJ];
         unsigned lane_sx[SCALED ? TI : 1], lane_sy[SCALED ? TJ : 1];  // this lane's scales of steps 0 and 1 in the low bytes
@@ -393,23 +488,20 @@ void k_grouped_tile(grouped_params p)
         if (!late_group) __builtin_amdgcn_s_barrier();
     }
 
-    // Neighbouring lanes hold neighbouring rows: they exchange the results of two MFMA tiles, so that a row's 32 go out together
-    // (128 bytes of Float32) from eight lanes, first the even rows and then the odd ones.
-    DT *D = (DT *)p.D + (SUM ? (long)at.group * p.sd : 0);
-    const int end_j = SUM ? p.J : at.last;
-    const bool odd = r & 1;
-#pragma unroll
-    for (int b = 0; b < TJ; b++) {
-        const int j = at.j0 + wj * WTJ + 16 * b + (r & ~1);
-        DT *row = D + (long)j * p.ldd;
-#pragma unroll
-        for (int a = 0; a < TI; a += 2) {
-            float4_t v0 = acc[a][b], v1 = acc[a + 1][b];
-            pair_exchange(odd, v0, v1);
-            const int i = at.i0 + wi * WTI + 16 * (a + odd) + 4 * q;
-            if (j < end_j) store_results<DT>(p, row, i, v0);
-            if (j + 1 < end_j) store_results<DT>(p, row + p.ldd, i, v1);
-        }
+    const grouped_tile done = at;
+    const bool more = WALKS && tile.at.group >= 0;
+    if (more) {
+        start(tile);
+        workgroup += (int)gridDim.x;
+        tile = find(workgroup);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const bool whole = store_tile(done);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!more) break;
+    // (the stores of a whole tile, younger than the requests, may stay in flight)
+    if (whole) wait_loads_and_barrier<TI * TJ>();
+    else wait_loads_and_barrier<0>();
     }
 }
 

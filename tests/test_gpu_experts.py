@@ -270,6 +270,57 @@ def test_grouped_wgrad_infinities_stay_in_their_group(gpu, rows, groups, m, n):
             assert np.array_equal(got[g], exact)
 
 
+# Products large enough for every tile, with edges on all sides and groups of very different size; whole numbers, so that the results
+# are exact whatever the order of the sums.
+def _large_groups(groups, rows):
+    if groups == 1:
+        return np.array([0, rows], np.int32)
+    cut = (np.arange(groups + 1) / groups) ** 1.7 * (rows - 5)
+    offsets = np.concatenate([[0], np.floor(cut[1:]) + 3]).astype(np.int32)
+    offsets[1] = offsets[0] = 2  # (the first group has no rows, and the last ones have no group)
+    return offsets
+
+
+@pytest.mark.parametrize("layout", ["col", "row"])
+@pytest.mark.parametrize("rows,groups,n,k,kind,out", [
+    (4000, 1, 4088, 72, "f16", "f16"), (8150, 3, 8184, 136, "bf16", "f32"), (2900, 3, 4096, 1000, "f16", "f32"), (1000, 4, 2056, 328, "bf16", "bf16"), (500, 12, 1032, 200, "f16", "f16")])
+def test_grouped_gemm_large(gpu, rows, groups, n, k, kind, out, layout):
+    rng = np.random.default_rng(rows)
+    kind, okind = KINDS[kind], KINDS[out]
+    offsets = _large_groups(groups, rows)
+    a_rows = rows // 2 + 7
+    gather = rng.integers(0, a_rows, rows).astype(np.int32)
+    a, w = rng.integers(-1, 2, (a_rows, k)).astype(np.float32), rng.integers(-1, 2, (groups, k, n)).astype(np.float32)
+    D = upload(gpu, np.full((rows, n), 99, okind.dtype))
+    gpu.EXPERTS.grouped_gemm(upload(gpu, kind.store(a)), upload(gpu, kind.store(w.transpose(0, 2, 1) if layout == "col" else w)), D, upload(gpu, offsets), rows=rows,
+                             groups=groups, n=n, k=k, dtype=kind.marker(gpu), d_type=okind.marker(gpu), gather=upload(gpu, gather), a_rows=a_rows,
+                             w_layout=gpu.WMMA.ColMajor if layout == "col" else gpu.WMMA.RowMajor)
+    got = D.to_host().reshape(rows, n)
+    for g in range(groups):
+        r = slice(offsets[g], offsets[g + 1])
+        assert np.array_equal(got[r], okind.store(a[gather[r]] @ w[g])), g
+    assert np.all(got[:offsets[0]] == 99) and np.all(got[offsets[-1]:] == 99)
+
+
+@pytest.mark.parametrize("rows,groups,m,n,kind,out", [(150, 1, 3496, 3592, "bf16", "f32"), (700, 3, 1992, 2056, "f16", "f32"), (900, 5, 1000, 1032, "bf16", "bf16"), (3000, 1, 520, 264, "f16", "f32")])
+def test_grouped_wgrad_large(gpu, rows, groups, m, n, kind, out):
+    rng = np.random.default_rng(rows)
+    kind, okind = KINDS[kind], KINDS[out]
+    offsets = _large_groups(groups, rows)
+    b_rows = rows // 2 + 7
+    gather = rng.integers(0, b_rows, rows).astype(np.int32)
+    a, b = rng.integers(-1, 2, (rows, m)).astype(np.float32), rng.integers(-1, 2, (b_rows, n)).astype(np.float32)
+    D = upload(gpu, np.full((groups, m, n), 99, okind.dtype))
+    args = upload(gpu, kind.store(a)), upload(gpu, kind.store(b)), D, upload(gpu, offsets)
+    sizes = dict(rows=rows, groups=groups, m=m, n=n, dtype=kind.marker(gpu), d_type=okind.marker(gpu), gather=upload(gpu, gather), b_rows=b_rows)
+    gpu.EXPERTS.grouped_wgrad(*args, **sizes)
+    want = np.stack([a[offsets[g]:offsets[g + 1]].T @ b[gather[offsets[g]:offsets[g + 1]]] for g in range(groups)])
+    assert np.array_equal(D.to_host().reshape(groups, m, n), okind.store(want))
+    if out == "f32":
+        gpu.EXPERTS.grouped_wgrad(*args, accumulate=True, **sizes)
+        assert np.array_equal(D.to_host().reshape(groups, m, n), 2 * want)
+
+
 def test_grouped_gemm_offsets_and_gather_outside(gpu):
     """Offsets and rows that lie outside are taken as the nearest inside: nothing else is read or written."""
     rng = np.random.default_rng(1)
@@ -433,6 +484,33 @@ def test_mxfp4_grouped_gemm(gpu, rows, groups, n, k, epilogue):
             want = ref.gated(exact)
         error = (k + 2) * 2.0 ** -24 * (1.1 * size[:, 0::2] * np.abs(exact[:, 1::2]) + np.abs(exact[:, 0::2]) * size[:, 1::2])
         assert np.all(np.abs(got - want)[inside] <= (error + 64 * 2.0 ** -23 * (1 + np.abs(exact[:, 0::2])) * np.abs(want) + 2.0 ** -25)[inside])
+
+
+@pytest.mark.parametrize("rows,groups,n,k", [(4000, 1, 4088, 600), (2900, 3, 4096, 1000), (1000, 4, 2056, 328), (500, 12, 1032, 2080), (16, 1, 4096, 1120)])
+def test_mxfp4_grouped_gemm_large(gpu, rows, groups, n, k):
+    """Whole numbers of magnitude 0 to 2 and scales of 1, 2 and 4: exact in Float32."""
+    Q, rng = gpu.MXFP4, np.random.default_rng(rows)
+    offsets = _large_groups(groups, rows)
+    a_rows = rows // 2 + 7
+    gather = rng.integers(0, a_rows, rows).astype(np.int32)
+
+    def matrix(rows):
+        blocks = -(-k // 32)
+        value = rng.choice(np.array([0, 2, 4, 8 + 2, 8 + 4], np.uint8), (rows, 32 * blocks))
+        value[:, k:] = 0
+        scales = rng.integers(127, 130, (rows, blocks)).astype(np.uint8)
+        x = np.where(value & 8, -1, 1) * ref.E2M1[value & 7] * np.exp2(np.repeat(scales.astype(np.float32), 32, 1) - 127)
+        return (value[:, 0::2] | value[:, 1::2] << 4).astype(np.uint8), ref.panels(scales, fill=255), x[:, :k].astype(np.float32)
+
+    a, w = matrix(a_rows), [matrix(n) for _ in range(groups)]
+    D = upload(gpu, np.full((rows, n), 99, np.float32))
+    Q.grouped_gemm(upload(gpu, a[0]), upload(gpu, a[1]), upload(gpu, np.stack([x[0] for x in w])), upload(gpu, np.stack([x[1] for x in w])), D, upload(gpu, offsets), rows=rows,
+                   groups=groups, n=n, k=k, d_type=np.float32, gather=upload(gpu, gather), a_rows=a_rows)
+    got = D.to_host().reshape(rows, n)
+    for g in range(groups):
+        r = slice(offsets[g], offsets[g + 1])
+        assert np.array_equal(got[r], a[2][gather[r]] @ w[g][2].T), g
+    assert np.all(got[:offsets[0]] == 99) and np.all(got[offsets[-1]:] == 99)
 
 
 def test_mxfp4_scales_that_stand_for_nan(gpu):
