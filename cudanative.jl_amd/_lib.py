@@ -161,6 +161,8 @@ SIGNATURES = {
     "miw_route_grad": (_i, [_i, _i64, _i, _i, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "miw_grouped_gemm": (_i, [_i, _i, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "miw_grouped_wgrad": (_i, [_i, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "miw_gated_silu": (_i, [_i, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "miw_gated_silu_grad": (_i, [_i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "miw_combine": (_i, [_i, _i64, _i, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "miw_combine_grad": (_i, [_i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "miw_mxfp4_quantize": (_i, [_i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),

@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmiwmma.so")
 SOURCES = ["gemm_tile_256x128.hip", "gemm_tile_256x256_w2x2.hip", "gemm_tile_small.hip", "gemm_tile_pp.hip", "gemm_tile_pp64.hip", "gemm_tile_wave128.hip",
            "capi.hip", "frag_kernels.hip", "gemm_skinny.hip", "gemm_kwave.hip", "gemm_kernels.hip",
-           "capi_experts.hip", "route.hip", "combine.hip", "mxfp4_convert.hip", "grouped_plain.hip",
+           "capi_experts.hip", "route.hip", "combine.hip", "gated.hip", "mxfp4_convert.hip", "grouped_plain.hip",
            "grouped_tile_f16.hip", "grouped_tile_bf16.hip", "grouped_tile_mxfp4.hip", "grouped_narrow.hip", "grouped_dispatch.hip"]
 
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")

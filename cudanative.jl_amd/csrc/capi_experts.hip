@@ -78,6 +78,14 @@ int check_epilogue(const char *what, int epilogue, int64_t n)
     return 0;
 }
 
+int check_gated(const char *what, int dtype, int64_t rows, int64_t n)
+{
+    if (!half_type(dtype)) return api_fail(MIW_ERR_INVALID_TYPE, "%s: unknown element type %d", what, dtype);
+    CHECK(check_extent(what, "rows", rows, 0, POSITIONS));
+    CHECK(check_extent(what, "n", n, 2, EXTENT));
+    return check_epilogue(what, MIW_EPILOGUE_GATED_SILU, n);
+}
+
 // Codes and scales of rows x k values; *ldq, *lds become the pitches that count.
 int check_mxfp4(const char *what, int64_t rows, int64_t k, int64_t *ldq, int64_t *lds, const void *codes, const void *scales)
 {
@@ -331,6 +339,57 @@ int miw_combine_grad(int dtype, int64_t tokens, int top, int64_t n, int64_t rows
     p.lddh = lddh;
     p.vector = aligned(dY, 16) && aligned(dH, 16) && (!dgates || aligned(H, 16)) && n % 8 == 0 && ldh % 8 == 0 && ldy % 8 == 0 && lddh % 8 == 0;
     HIP_TRY(miw::launch_combine_grad(p, dtype, (hipStream_t)stream));
+    return 0;
+}
+
+int miw_gated_silu(int dtype, int64_t rows, int64_t n, int64_t ldz, int64_t lda, const void *Z, void *A, void *stream)
+{
+    const char *what = "gated_silu";
+    CHECK(check_gated(what, dtype, rows, n));
+    CHECK(check_pitch(what, "ldz", &ldz, n));
+    CHECK(check_pitch(what, "lda", &lda, n / 2));
+    if (!rows) return 0;
+    CHECK(check_element(what, "Z", Z, 2));
+    CHECK(check_element(what, "A", A, 2));
+    REQUIRE_INIT(what);
+    miw::gated_params p{};
+    p.Z = Z;
+    p.out = A;
+    p.rows = rows;
+    p.n = n;
+    p.ldz = ldz;
+    p.ldo = lda;
+    p.vector = aligned(Z, 16) && aligned(A, 8) && n % 8 == 0 && ldz % 8 == 0 && lda % 4 == 0;
+    HIP_TRY(miw::launch_gated_silu(p, dtype, (hipStream_t)stream));
+    return 0;
+}
+
+int miw_gated_silu_grad(int dtype, int64_t rows, int64_t n, int64_t ldz, int64_t ldda, int64_t lddz, const void *Z, const void *dA,
+                        void *dZ, void *stream)
+{
+    const char *what = "gated_silu_grad";
+    CHECK(check_gated(what, dtype, rows, n));
+    CHECK(check_pitch(what, "ldz", &ldz, n));
+    CHECK(check_pitch(what, "ldda", &ldda, n / 2));
+    CHECK(check_pitch(what, "lddz", &lddz, n));
+    if (!rows) return 0;
+    CHECK(check_element(what, "Z", Z, 2));
+    CHECK(check_element(what, "dA", dA, 2));
+    CHECK(check_element(what, "dZ", dZ, 2));
+    if (dZ == Z && lddz != ldz)
+        return api_fail(MIW_ERR_INVALID_VALUE, "%s: dZ in Z's place needs Z's pitch, got %lld and %lld", what, (long long)lddz, (long long)ldz);
+    REQUIRE_INIT(what);
+    miw::gated_params p{};
+    p.Z = Z;
+    p.dA = dA;
+    p.out = dZ;
+    p.rows = rows;
+    p.n = n;
+    p.ldz = ldz;
+    p.ldda = ldda;
+    p.ldo = lddz;
+    p.vector = aligned(Z, 16) && aligned(dA, 8) && aligned(dZ, 16) && n % 8 == 0 && ldz % 8 == 0 && ldda % 4 == 0 && lddz % 8 == 0;
+    HIP_TRY(miw::launch_gated_silu(p, dtype, (hipStream_t)stream));
     return 0;
 }
 

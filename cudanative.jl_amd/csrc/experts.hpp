@@ -47,6 +47,16 @@ struct combine_params {
 hipError_t launch_combine(const combine_params &p, int dtype, hipStream_t s);
 hipError_t launch_combine_grad(const combine_params &p, int dtype, hipStream_t s);
 
+// --- gated.hip
+struct gated_params {
+    const void *Z, *dA;  // dA null: the forward pass
+    void *out;           // A, or dZ
+    long rows, n, ldz, ldda, ldo;
+    int vector;       // 16-byte accesses to Z and dZ, 8-byte ones to A and dA
+    int column_bits;  // set by the launch
+};
+hipError_t launch_gated_silu(gated_params p, int dtype, hipStream_t s);
+
 // --- mxfp4_convert.hip
 struct mxfp4_convert_params {
     const void *in;

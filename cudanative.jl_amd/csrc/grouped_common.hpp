@@ -93,7 +93,6 @@ inline long grouped_blocks(const grouped_params &p, long bi, long bj, long threa
     return n * threads < (1l << 32) && n < (1l << 30) ? n : 0;
 }
 
-__device__ inline float gated_silu(float gate, float value) { return gate / (1.f + __expf(-gate)) * value; }
 
 // Stores the four results i .. i + 3 of row j; those from I on are left out.  In the gated form they are two pairs of gate and
 // value, and two results are stored (I counts the columns before that).

@@ -52,6 +52,10 @@ __device__ inline void store8(T *p, f32x8 v, int count)
     }
 }
 
+// The gate of a gated SiLU times its value.  (__expf is within a few units of Float32's last place over the range in which the
+// result is not a zero, far below the rounding that follows.)
+__device__ inline float gated_silu(float gate, float value) { return gate / (1.f + __expf(-gate)) * value; }
+
 // Reductions over a wavefront by data-parallel primitives: no LDS, some fifty cycles.  The result is uniform.
 __device__ inline unsigned wave_max(unsigned v)
 {

@@ -1,8 +1,8 @@
 """A layer of experts: routing, products grouped by expert, the join of the answers, and the gradients.
 
 Every token goes to a few of many matrices.  `route` chooses them and sorts the rows by expert, `grouped_gemm` multiplies
-each expert's rows by its matrix, `combine` joins a token's answers by its gates; `route_grad`, `grouped_wgrad` and
-`combine_grad` are the way back.  How many rows an expert has stays on the device: nothing here waits for it.
+each expert's rows by its matrix, `combine` joins a token's answers by its gates; `route_grad`, `grouped_wgrad`,
+`gated_silu_grad` and `combine_grad` are the way back.  How many rows an expert has stays on the device: nothing here waits for it.
 
 No counterpart in the reference; the products are the chain of mma calls of docs/src/device/wmma.md:51-52 on ragged
 rows.  Arrays are DeviceArrays or raw device addresses; matrices are row-major, a pitch or stride of 0 means dense.  All
@@ -97,6 +97,16 @@ def grouped_wgrad(A, B, D, offsets, *, rows, groups, m, n, dtype=Float16, d_type
     accumulate: added to D."""
     _check(_library.miw_grouped_wgrad(type_code(dtype), type_code(d_type), 1 if accumulate else 0, rows, groups, m, n, lda, ldb, ldd, stride_d, b_rows,
                                              _ptr(A), _ptr(B), _ptr(D), _ptr(offsets), _ptr(gather), None if stream is None else _stream(stream)))
+
+
+def gated_silu(Z, A, *, rows, n, dtype=Float16, ldz=0, lda=0, stream=None):
+    """A (rows x n / 2) = silu(columns 2c) * (columns 2c + 1) of Z (rows x n): what the epilogue GATED_SILU does, from stored columns."""
+    _check(_library.miw_gated_silu(type_code(dtype), rows, n, ldz, lda, _ptr(Z), _ptr(A), None if stream is None else _stream(stream)))
+
+
+def gated_silu_grad(Z, dA, dZ, *, rows, n, dtype=Float16, ldz=0, ldda=0, lddz=0, stream=None):
+    """The gradient to Z from the one to A; dZ may be Z."""
+    _check(_library.miw_gated_silu_grad(type_code(dtype), rows, n, ldz, ldda, lddz, _ptr(Z), _ptr(dA), _ptr(dZ), None if stream is None else _stream(stream)))
 
 
 def combine(H, place, Y, *, tokens, top, n, rows, dtype=Float16, gates=None, ldh=0, ldy=0, stream=None):

@@ -31,7 +31,7 @@ module MIWMMA
 export DeviceBuffer, DevicePtr, AS, WMMA, @hip, gemm!, gemm_splitk!, gemm_splitk_static!, synchronize, MIWError,
        HostKernel, hipfunction, CodeObject, kernel, registers, memory, maxthreads, launch_configuration,
        Stream, device_info, warpsize, nextwarp, prevwarp, mem_info,
-       route!, route_grad!, grouped_gemm!, grouped_wgrad!, combine!, combine_grad!,
+       route!, route_grad!, grouped_gemm!, grouped_wgrad!, gated_silu!, gated_silu_grad!, combine!, combine_grad!,
        mxfp4_quantize!, mxfp4_dequantize!, mxfp4_gemm!, mxfp4_grouped_gemm!
 
 const libmiwmma = get(ENV, "MIWMMA_LIB", joinpath(@__DIR__, "..", "libmiwmma.so"))
@@ -876,6 +876,21 @@ function grouped_wgrad!(D, A, B, offsets; rows::Integer, groups::Integer, m::Int
         ELEMENT_CODES[dtype], ELEMENT_CODES[d_type], accumulate ? 1 : 0, rows, groups, m, n, lda, ldb, ldd, stride_d, b_rows,
         address(A), address(B), address(D), address(offsets), address(gather), stream_handle(stream)))
     return D
+end
+
+"A (rows x n / 2) = silu(columns 2c) * (columns 2c + 1) of Z (rows x n)."
+function gated_silu!(A, Z; rows::Integer, n::Integer, dtype::Symbol=:f16, ldz::Integer=0, lda::Integer=0, stream=C_NULL)
+    GC.@preserve A Z check(ccall((:miw_gated_silu, libmiwmma), Cint, (Cint, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], rows, n, ldz, lda, address(Z), address(A), stream_handle(stream)))
+    return A
+end
+
+function gated_silu_grad!(dZ, Z, dA; rows::Integer, n::Integer, dtype::Symbol=:f16, ldz::Integer=0, ldda::Integer=0, lddz::Integer=0,
+                          stream=C_NULL)
+    GC.@preserve dZ Z dA check(ccall((:miw_gated_silu_grad, libmiwmma), Cint,
+        (Cint, Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+        ELEMENT_CODES[dtype], rows, n, ldz, ldda, lddz, address(Z), address(dA), address(dZ), stream_handle(stream)))
+    return dZ
 end
 
 "Y[t] = sum over j of gates[t, j] * H[place[t, j]]."

@@ -345,6 +345,7 @@ int miw_copy_probe(void *dst, const void *src, size_t bytes, void *stream);
      miw_route         which experts a token goes to, with which weights, and where its rows lie in the sorted order
      miw_grouped_gemm  the rows of each expert times its matrix (forward pass, and gradient to the rows)
      miw_grouped_wgrad the gradient to each expert's matrix
+     miw_gated_silu    the activation between two products, where training keeps both sides of it
      miw_combine       a token's answers joined by its weights
    Nothing here waits for the device: how many rows an expert has is only known there, and stays there (`offsets`).
    Matrices are row-major; a leading dimension or stride of 0 means "dense".  Element types: MIW_F16, MIW_BF16 and, where
@@ -386,8 +387,14 @@ int miw_grouped_wgrad(int dtype, int d_type, int accumulate, int64_t rows, int g
                       int64_t ldb, int64_t ldd, int64_t stride_d, int64_t b_rows, const void *A, const void *B, void *D,
                       const int *offsets, const int *gather, void *stream);
 
+/* The gated form by itself, for training, which keeps the columns Z (rows x n, n even) that a product without epilogue stored:
+   A (rows x n / 2) from Z, and Z's gradient from A's.  F16 or BF16, Float32 between a load and its rounding.  dZ may be Z itself. */
+int miw_gated_silu(int dtype, int64_t rows, int64_t n, int64_t ldz, int64_t lda, const void *Z, void *A, void *stream);
+int miw_gated_silu_grad(int dtype, int64_t rows, int64_t n, int64_t ldz, int64_t ldda, int64_t lddz, const void *Z, const void *dA,
+                        void *dZ, void *stream);
+
 /* Y[t] = sum over j of gates[t][j] * H[place[t][j]], in the order of j (gates null: 1, which joins gradients to rows that
-   were gathered).  A place outside 0 .. rows - 1 adds nothing.  H: rows x n, Y: tokens x n. */
+   were gathered).  A place outside 0 .. rows - 1 adds nothing.  H: rows x n, Y: tokens x n.  Fewer than 2^24 tokens. */
 int miw_combine(int dtype, int64_t tokens, int top, int64_t n, int64_t rows, int64_t ldh, int64_t ldy, const void *H,
                 const float *gates, const int *place, void *Y, void *stream);
 /* dH[place[t][j]] = gates[t][j] * dY[t] (rows that no place names are not touched), dgates[t][j] = dY[t] . H[place[t][j]]
