@@ -11,7 +11,7 @@
 // lower experts and earlier chunks and writes the positions.  Counts are integers: no order of theirs matters.
 //
 // Bound by latency throughout: 16381 tokens, 128 experts, 8 choices (bf16): 4.2 MB of logits, 1.6 MB of results:
-// choose 8.7 us, place 8.3 us, gradient 7.8 us (8.4 MB in and out) where the bytes alone take one to two each.  16 tokens of 64
+// choose 8.7 us, place 8.3 us, gradient 5.9 us (8.4 MB in and out; with a wavefront a token 7.8) where the bytes alone take one to two each.  16 tokens of 64
 // experts, 4 choices: one launch of 3.2 us.
 #include "experts.hpp"
 #include "vec_types.hpp"
@@ -300,60 +300,61 @@ __global__ __launch_bounds__(ROUTE_THREADS) void k_route_place(route_params p)
     for (int i = total + (int)(blockIdx.x * ROUTE_THREADS) + tid; i < p.tokens * p.top; i += (int)(gridDim.x * ROUTE_THREADS)) p.rows[i] = -1;
 }
 
-// dz over the chosen: g (dg - sum g dg); over all: p_e (dg_e - sum g dg), dg_e zero where e is not chosen.  A wavefront per token; its
-// logits, R registers a lane, are asked for together with what it chose.
-template <class T, int R>
+// dz over the chosen: g (dg - sum g dg); over all: p_e (dg_e - sum g dg), dg_e zero where e is not chosen.  LANES (16 up to 256 experts,
+// or 64) have a token; its logits, R registers a lane, are asked for together with what it chose.
+template <class T, int R, int LANES>
 __global__ __launch_bounds__(256) void k_route_grad(route_grad_params p)
 {
-    const int lane = threadIdx.x & 63, token = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (token >= p.tokens) return;
-    const T *z = (const T *)p.logits + (long)token * p.ld;
-    T *dz = (T *)p.dlogits + (long)token * p.ldd;
-    float v[R];
-    if (p.over_all)
+    const int lane = threadIdx.x & (LANES - 1);
+    for (long token = ((long)blockIdx.x * 256 + threadIdx.x) / LANES; token < p.tokens; token += (long)gridDim.x * (256 / LANES)) {
+        const T *z = (const T *)p.logits + token * p.ld;
+        T *dz = (T *)p.dlogits + token * p.ldd;
+        float v[R];
+        if (p.over_all)
 #pragma unroll
-        for (int i = 0; i < R; i++) v[i] = lane + 64 * i < p.experts ? (float)z[lane + 64 * i] : -__builtin_inff();
-    const long at = (long)token * p.top + lane;
-    int expert = -1;
-    float gate = 0.f, dgate = 0.f;
-    if (lane < p.top) {
-        expert = p.chosen[at];
-        gate = p.gates[at];
-        dgate = p.dgates[at];
-    }
-    if (expert < 0) gate = dgate = 0.f;  // (what a choice without an expert gets is not looked at)
-    const float inner = wave_sum(gate * dgate);
-    const float direct = p.over_all ? gate * dgate : gate * (dgate - inner);
-    float total = 1.f;
-    if (p.over_all) {
-        // The softmax over all logits from its largest.
-        unsigned most = 0;
-#pragma unroll
-        for (int i = 0; i < R; i++) most = max(most, order_key(v[i]));
-        most = wave_max(most);
-        const float largest = most ? fminf(key_value(most), LARGEST) : 0.f;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            v[i] = v[i] > -__builtin_inff() ? __expf(fminf(v[i], LARGEST) - largest) : 0.f;  // (NaN: 0)
-            sum += v[i];
+            for (int i = 0; i < R; i++) v[i] = lane + LANES * i < p.experts ? (float)z[lane + LANES * i] : -__builtin_inff();
+        const long at = token * p.top + lane;
+        int expert = -1;
+        float gate = 0.f, dgate = 0.f;
+        if (lane < p.top) {
+            expert = p.chosen[at];
+            gate = p.gates[at];
+            dgate = p.dgates[at];
         }
-        total = wave_sum(sum);
-        if (total == 0.f) total = 1.f;
-    }
-    float d[R];
+        if (expert < 0) gate = dgate = 0.f;  // (what a choice without an expert gets is not looked at)
+        const float inner = LANES == 16 ? row_sum(gate * dgate) : wave_sum(gate * dgate);
+        const float direct = p.over_all ? gate * dgate : gate * (dgate - inner);
+        float scale = 0.f;
+        if (p.over_all) {
+            // The softmax over all logits from its largest.
+            unsigned most = 0;
 #pragma unroll
-    for (int i = 0; i < R; i++) d[i] = p.over_all ? -(v[i] / total) * inner : 0.f;
-    for (int j = 0; j < p.top; j++) {
-        const int x = __builtin_amdgcn_readlane(expert, j);
-        const float add = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, direct), j));
+            for (int i = 0; i < R; i++) most = max(most, order_key(v[i]));
+            most = LANES == 16 ? row_max(most) : wave_max(most);
+            const float largest = most ? fminf(key_value(most), LARGEST) : 0.f;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                v[i] = v[i] > -__builtin_inff() ? __expf(fminf(v[i], LARGEST) - largest) : 0.f;  // (NaN: 0)
+                sum += v[i];
+            }
+            const float total = LANES == 16 ? row_sum(sum) : wave_sum(sum);
+            if (total > 0.f) scale = -inner / total;
+        }
+        float d[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) d[i] = p.over_all ? v[i] * scale : 0.f;
+        for (int j = 0; j < p.top; j++) {
+            const int x = __shfl(expert, j, LANES);
+            const float add = __shfl(direct, j, LANES);
+            const int hit = (x & (LANES - 1)) == lane ? x >> (LANES == 16 ? 4 : 6) : -1;  // (-1 stays -1)
+#pragma unroll
+            for (int i = 0; i < R; i++) d[i] += hit == i ? add : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < R; i++)
-            if (x == lane + 64 * i) d[i] += add;
+            if (lane + LANES * i < p.experts) dz[lane + LANES * i] = (T)d[i];
     }
-#pragma unroll
-    for (int i = 0; i < R; i++)
-        if (lane + 64 * i < p.experts) dz[lane + 64 * i] = (T)d[i];
 }
 
 // At most 256 chunks of sixteen tokens (one a wavefront) or more; one workgroup as long as it has its tokens together.
@@ -407,11 +408,15 @@ hipError_t launch_route(route_params p, int dtype, hipStream_t s)
 
 hipError_t launch_route_grad(const route_grad_params &p, int dtype, hipStream_t s)
 {
-    const dim3 grid((unsigned)((p.tokens + 3) / 4)), block(256);
+    const bool row = p.experts <= 256;
+    const long blocks = (p.tokens + (row ? 15l : 3l)) / (row ? 16 : 4);
+    const dim3 grid((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), block(256);
     with_type(dtype, [&](auto type) {
-        with_registers(p.experts, [&](auto regs) {
-            hipLaunchKernelGGL((k_route_grad<decltype(type), decltype(regs)::value>), grid, block, 0, s, p);
+        using T = decltype(type);
+        if (row) with_registers(p.experts, [&](auto regs) {
+            hipLaunchKernelGGL((k_route_grad<T, 4 * (decltype(regs)::value < 4 ? decltype(regs)::value : 4), 16>), grid, block, 0, s, p);
         });
+        else hipLaunchKernelGGL((k_route_grad<T, 16, 64>), grid, block, 0, s, p);
     });
     return hipGetLastError();
 }
