@@ -9,6 +9,10 @@ namespace miw {
 // Element types, numbered as MIW_F16, MIW_F32, MIW_BF16.
 enum { TYPE_F16 = 0, TYPE_F32 = 1, TYPE_BF16 = 2 };
 
+// A matrix of more than this is streamed past the caches by the kernels that touch every element once: it, the result and what
+// the calls before and after work on no longer share the last-level cache (256 MiB).  Each kernel says what it measured.
+constexpr long STREAM_BYTES = 96l << 20;
+
 // --- route.hip
 struct route_params {
     const void *logits;

@@ -3,8 +3,8 @@
 // A lane has eight values of a block, four lanes the block, 32 lanes a row's piece of one panel of scales (256 values); the
 // largest magnitude meets in the four lanes by data-parallel moves.  The scale is a power of two, so dividing by it is
 // exact, and v_cvt_scalef32_pk_fp4_f32 rounds to the nearest code, ties to the even one, and saturates.
-// Bound by HBM: a Float16 matrix is read once (2 bytes a value) and 17/32 of a byte written.  8192 x 8192 (Float16): 39 us
-// (170 MB, 4.4 TB/s), back to bfloat16 26 us (170 MB, 6.6 TB/s: the codes are still in a cache).
+// Bound by HBM: a Float16 matrix is read once (2 bytes a value) and 17/32 of a byte written.  8192 x 8192 (Float16): 33 us
+// (170 MB, 5.2 TB/s), back to bfloat16 25 us (170 MB, 6.8 TB/s: the codes are still in a cache).
 #include "experts.hpp"
 #include "vec_types.hpp"
 
@@ -15,7 +15,7 @@ constexpr int CONVERT_THREADS = 256;
 // 2^n for n in -127 .. 127.
 __device__ inline float power_of_two(int n) { return __builtin_ldexpf(1.f, n); }
 
-template <class T, bool VECTOR>
+template <class T, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(CONVERT_THREADS) void k_mxfp4_quantize(mxfp4_convert_params p)
 {
     const long panels = (p.k + 255) / 256;
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(CONVERT_THREADS) void k_mxfp4_quantize(mxfp4_conver
         const long k0 = panel * 256 + sub * 8;
         const int count = (int)max(0l, min(8l, p.k - k0));
         f32x8 v = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (count == 8) v = load8<T, VECTOR>((const T *)p.in + row * p.ld + k0, 8);
+        if (count == 8) v = load8<T, VECTOR, STREAM>((const T *)p.in + row * p.ld + k0, 8);
         else if (count > 0) v = load8<T, false>((const T *)p.in + row * p.ld + k0, count);
         // Magnitudes as unsigned numbers have their order, infinities and NaN above all others.
         unsigned most = 0;
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(CONVERT_THREADS) void k_mxfp4_quantize(mxfp4_conver
     }
 }
 
-template <class T, bool VECTOR>
+template <class T, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(CONVERT_THREADS) void k_mxfp4_dequantize(mxfp4_convert_params p)
 {
     const long eights = (p.k + 7) / 8;
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(CONVERT_THREADS) void k_mxfp4_dequantize(mxfp4_conv
         const float by = scale == 255 ? __builtin_nanf("") : power_of_two(scale - 127);
         const f32x8 v = {a[0] * by, a[1] * by, b[0] * by, b[1] * by, c[0] * by, c[1] * by, d[0] * by, d[1] * by};
         T *to = (T *)p.out + row * p.ld + k0;
-        if (count == 8) store8<T, VECTOR>(to, v, 8);
+        if (count == 8) store8<T, VECTOR, STREAM>(to, v, 8);
         else store8<T, false>(to, v, count);
     }
 }
@@ -86,6 +86,11 @@ static hipError_t typed(int dtype, F go)
     else go(bf16_t{});
     return hipGetLastError();
 }
+// The matrix streams past the caches, codes and scales stay.  Writing X, its codes, reading them, back, reading that, 8192 columns (bf16),
+// streamed and not: 338 and 387 us at 268 MB of X, 178 and 195 at 134 MB; 101 and 99 at 67 MB.
+template <class T>
+static bool streams(const mxfp4_convert_params &p) { return p.vector && (long)sizeof(T) * p.rows * p.k > STREAM_BYTES; }
+
 static dim3 convert_grid(long threads)
 {
     const long blocks = (threads + CONVERT_THREADS - 1) / CONVERT_THREADS;
@@ -97,8 +102,9 @@ hipError_t launch_mxfp4_quantize(const mxfp4_convert_params &p, int dtype, hipSt
     const dim3 grid = convert_grid((p.k + 255) / 256 * 32 * p.rows), block(CONVERT_THREADS);
     return typed(dtype, [&](auto type) {
         using T = decltype(type);
-        if (p.vector) hipLaunchKernelGGL((k_mxfp4_quantize<T, true>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((k_mxfp4_quantize<T, false>), grid, block, 0, s, p);
+        if (streams<T>(p)) hipLaunchKernelGGL((k_mxfp4_quantize<T, true, true>), grid, block, 0, s, p);
+        else if (p.vector) hipLaunchKernelGGL((k_mxfp4_quantize<T, true, false>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((k_mxfp4_quantize<T, false, false>), grid, block, 0, s, p);
     });
 }
 
@@ -107,8 +113,9 @@ hipError_t launch_mxfp4_dequantize(const mxfp4_convert_params &p, int dtype, hip
     const dim3 grid = convert_grid((p.k + 7) / 8 * p.rows), block(CONVERT_THREADS);
     return typed(dtype, [&](auto type) {
         using T = decltype(type);
-        if (p.vector) hipLaunchKernelGGL((k_mxfp4_dequantize<T, true>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((k_mxfp4_dequantize<T, false>), grid, block, 0, s, p);
+        if (streams<T>(p)) hipLaunchKernelGGL((k_mxfp4_dequantize<T, true, true>), grid, block, 0, s, p);
+        else if (p.vector) hipLaunchKernelGGL((k_mxfp4_dequantize<T, true, false>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((k_mxfp4_dequantize<T, false, false>), grid, block, 0, s, p);
     });
 }
 

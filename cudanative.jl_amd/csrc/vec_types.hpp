@@ -15,15 +15,29 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <class T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
 
+// A whole vector; STREAM: the caches are told that it is not used again soon.
+template <bool STREAM, class V>
+__device__ inline V load_vector(const V *p)
+{
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool STREAM, class V>
+__device__ inline void store_vector(V *p, V v)
+{
+    if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
 // Eight consecutive elements as Float32; VECTOR: one or two 16-byte loads, otherwise `count` single ones and zeros behind them.
-template <class T, bool VECTOR>
+template <class T, bool VECTOR, bool STREAM = false>
 __device__ inline f32x8 load8(const T *p, int count)
 {
     if constexpr (VECTOR) {
         if constexpr (sizeof(T) == 2) {
-            return __builtin_convertvector(*(const vec<T, 8> *)p, f32x8);
+            return __builtin_convertvector(load_vector<STREAM>((const vec<T, 8> *)p), f32x8);
         } else {
-            const f32x4 a = ((const f32x4 *)p)[0], b = ((const f32x4 *)p)[1];
+            const f32x4 a = load_vector<STREAM>((const f32x4 *)p), b = load_vector<STREAM>((const f32x4 *)p + 1);
             return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         }
     } else {
@@ -35,15 +49,15 @@ __device__ inline f32x8 load8(const T *p, int count)
     }
 }
 // Rounded to T (nearest, ties to even) and stored.
-template <class T, bool VECTOR>
+template <class T, bool VECTOR, bool STREAM = false>
 __device__ inline void store8(T *p, f32x8 v, int count)
 {
     if constexpr (VECTOR) {
         if constexpr (sizeof(T) == 2) {
-            *(vec<T, 8> *)p = __builtin_convertvector(v, vec<T, 8>);
+            store_vector<STREAM>((vec<T, 8> *)p, __builtin_convertvector(v, vec<T, 8>));
         } else {
-            ((f32x4 *)p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-            ((f32x4 *)p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+            store_vector<STREAM>((f32x4 *)p, f32x4{v[0], v[1], v[2], v[3]});
+            store_vector<STREAM>((f32x4 *)p + 1, f32x4{v[4], v[5], v[6], v[7]});
         }
     } else {
 #pragma unroll
