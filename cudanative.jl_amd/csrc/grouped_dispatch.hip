@@ -1,9 +1,9 @@
 // Which kernel runs a product grouped by expert.
 //
-// How many rows a group has is not known on the host: the rules go by the mean, rows / groups.  Their numbers come from 222
-// products timed on every kernel (1 to 128 groups, 1024 to 4096 wide, 0.5 to 2048 rows a group whose loads differ by up to three
-// times, f16 and 4 bits, weights from HBM): the rule's kernel takes 1.01 (f16) and 1.02 (4 bits) of the fastest one's time in the
-// geometric mean.
+// How many rows a group has is not known on the host: the rules go by the mean, rows / groups.  Their numbers come from some 400
+// products timed on every kernel (1 to 128 groups, 512 to 4096 wide, 0.5 to 2048 rows a group whose loads differ by up to three
+// times, f16 with k or i contiguous in the weights and 4 bits, weights from HBM): the rule's kernel takes 1.01 (f16) and 1.02 (4 bits)
+// of the fastest one's time in the geometric mean, at worst 1.38 (8 groups of 384 rows in the mean, whose real loads make whole rounds).
 #include "experts.hpp"
 
 #include <algorithm>
@@ -64,13 +64,16 @@ static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int
     return best->size;
 }
 
-// A ragged sum writes every group's whole result, and the largest tile reads the operands least often: taken as soon as its tiles fill
-// three quarters of the CUs, as the next one is (16 groups of 128 rows, 2048 x 4096: 143 us, 165 on 256 x 128; one group of 2048 rows, 1024
-// x 1024, which is 16 of the largest tiles: 48.3 us, 22.5 on 128 x 64).
+// A ragged sum writes every group's whole result, and the larger a tile the less often the operands are read: the largest one whose tiles fill
+// three quarters of the CUs.  Up to 1500 rows a group the tile's start and end count more than that, and 256 x 128 with slots of 32,
+// of which a CU holds two workgroups, comes first (16 groups, 2048 x 4096, Float32: 128 rows 142 us, 154 on 256 x 256; 512 rows 236 and 258;
+// but 8 groups of 2048 rows, 4096 x 4096: 618 and 560.  One group of 2048 rows, 1024 x 1024, 16 of the largest tiles: 47 us, 22 on 128 x 64).
 static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
 {
-    for (const tile_price &t : g_tiles)
+    for (const tile_price &t : g_tiles) {
+        if (t.size == TILE_256x256 && p.rows < 1500l * p.groups) continue;
         if (p.groups * ceil_div(p.I, t.bi) * ceil_div(p.J, t.bj) >= 3l * cus / 4) return t.size;
+    }
     return TILE_128x64;
 }
 

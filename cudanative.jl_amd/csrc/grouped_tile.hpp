@@ -9,15 +9,21 @@
 //   Ragged rows: Y's rows are a tile of one group's, through gather; the lanes' addresses are full ones.  Rows behind the
 //     group's last repeat it and are not stored.  X is the group's weights, k contiguous or i contiguous.
 //   Ragged sum: both operands have i (j) contiguous and k runs over a group's rows.  X's rows come through gather, whose
-//     entries travel to LDS NSLOT - 1 slots ahead of the slot that they are for.
+//     entries travel to LDS NY - 1 slots ahead of the slot that they are for.  A slot is 64 along k, or 32, where half the LDS then
+//     suffices for a tile of 256 x 128 and a CU holds two workgroups: while one waits for its first slot the other multiplies.  Stores
+//     and products add up all the same: 8198 rows, 16 groups, 2048 x 4096 (bf16, Float32 results): without stores 136 to 147 us, stores
+//     alone 111 to 118, both 238 to 258 on 256 x 256 with slots of 64; 224 to 236 on 256 x 128 with slots of 32.
 // Where the sum ends inside a slot, lanes fetch the last valid chunk (row) again and its values are zeroed in both operands'
 // fragments, in a copy of the loop body that only the last slot runs.
 #pragma once
 #include "grouped_common.hpp"
 
+#include <type_traits>
+
 namespace miw {
 
-enum grouped_form { ROWS_X_K = 0, ROWS_X_I = 1, RAGGED_SUM = 2 };
+enum grouped_form { ROWS_X_K = 0, ROWS_X_I = 1, RAGGED_SUM = 2, RAGGED_SUM_32 = 3 };  // (the last: in slots of 32 along k)
+constexpr bool grouped_sums(int form) { return form >= RAGGED_SUM; }
 
 struct op_f16 : mfma_f16 {
     static constexpr bool scaled = false;
@@ -45,10 +51,10 @@ __device__ inline void lds_load4(const char *lane_address, unsigned lds_base)
 }
 
 // A slot of one operand: its rows' 128 bytes, then their scales.
-constexpr int grouped_slot_bytes(int rows, bool scaled) { return rows * (128 + (scaled ? 8 : 0)); }
+constexpr int grouped_slot_bytes(int rows, bool scaled, int form) { return rows * ((form == RAGGED_SUM_32 ? 64 : 128) + (scaled ? 8 : 0)); }
 constexpr int grouped_lds_bytes(int bi, int bj, int nx, int ny, bool scaled, int form)
 {
-    return nx * grouped_slot_bytes(bi, scaled) + ny * grouped_slot_bytes(bj, scaled) + (form == RAGGED_SUM ? 2 * ny * 256 : 0);
+    return nx * grouped_slot_bytes(bi, scaled, form) + ny * grouped_slot_bytes(bj, scaled, form) + (grouped_sums(form) ? 2 * ny * 256 : 0);
 }
 
 // Workgroups that a CU holds together.
@@ -57,7 +63,7 @@ constexpr int grouped_workgroups(int bi, int bj, int nx, int ny, bool scaled, in
     return grouped_lds_bytes(bi, bj, nx, ny, scaled, form) <= 80 * 1024 ? 2 : 1;
 }
 // Do workgroups walk several tiles?
-constexpr bool grouped_walks(bool scaled, int form) { return !scaled && form != RAGGED_SUM; }
+constexpr bool grouped_walks(bool scaled, int form) { return !scaled && !grouped_sums(form); }
 
 // Tile of a ragged sum: groups one after the other, eight tiles along j together.
 template <class PARAMS>
@@ -74,6 +80,28 @@ __device__ inline grouped_tile find_sum_tile(const PARAMS &p, int bi, int bj, in
     const int i = in / height, j = band * GROUP_J_TILES + in - i * height;
     return {group, __builtin_amdgcn_readfirstlane(rows.first), __builtin_amdgcn_readfirstlane(rows.last), j * bj, i * bi};
 }
+
+// Fragments of a slot of 32 along k whose rows have i contiguous: as frag_reader, with 32 rows to each 64 along i.
+struct short_reader {
+    int base[4];
+    __device__ inline void init(int wave_row0, int lane)
+    {
+        const int j = lane & 15, q = lane >> 4, jq = j >> 2, jr = j & 3;
+        const int g = ((jq >> 1) & 1) | ((q & 1) << 1);  // i_major_swizzle of this lane's k
+        const int w16 = wave_row0 / 16;
+#pragma unroll
+        for (int m = 0; m < 4; m++) base[m] = (w16 / 4) * 4096 + (8 * q + jq) * 128 + jr * 8 + ((((w16 & 3) + m) & 3) ^ g) * 32;
+    }
+    template <int T, int H>
+    __device__ inline half8_t read(MIW_LDS const char *slot) const
+    {
+        static_assert(H == 0, "one step");
+        const int off = base[T & 3] + (T >> 2) * 4096;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((MIW_LDS fp16x4_t *)(slot + off)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((MIW_LDS fp16x4_t *)(slot + off + 512)));
+        return __builtin_bit_cast(half8_t, u32x4{lo[0], lo[1], hi[0], hi[1]});
+    }
+};
 
 // Zeroes the values of a lane's 16-byte fragment of 16-bit elements from `keep` on.
 __device__ inline void keep_first(u32x4 &f, int keep)
@@ -94,27 +122,31 @@ void k_grouped_tile(grouped_params p)
 {
     constexpr int NT = 512;
     static_assert(WI * WJ == 8, "two wavefronts per SIMD");
-    constexpr bool XK = FORM == ROWS_X_K, YK = FORM != RAGGED_SUM, SUM = FORM == RAGGED_SUM, SCALED = OP::scaled;
+    constexpr bool XK = FORM == ROWS_X_K, SUM = grouped_sums(FORM), YK = !SUM, SCALED = OP::scaled;
+    constexpr bool SHORT = FORM == RAGGED_SUM_32;
+    constexpr int SLOT_K = SHORT ? 32 : OP::slot_k, LOAD_I = SHORT ? 128 : 64;  // LOAD_I: rows of a tile that one load takes
     static_assert(!SCALED || XK, "4-bit operands have k contiguous");
     constexpr int WTI = BI / WI, WTJ = BJ / WJ, TI = WTI / 16, TJ = WTJ / 16;
-    constexpr int XBYTES = BI * 128, YBYTES = BJ * 128, XSLOT = grouped_slot_bytes(BI, SCALED), YSLOT = grouped_slot_bytes(BJ, SCALED);
+    constexpr int XBYTES = BI * 128, YBYTES = BJ * 128, XSLOT = grouped_slot_bytes(BI, SCALED, FORM), YSLOT = grouped_slot_bytes(BJ, SCALED, FORM);
     constexpr int XRING = NX * XSLOT, YRING = NY * YSLOT, INDEX = XRING + YRING;  // X's ring, Y's, that of the gathered rows
     static_assert(grouped_lds_bytes(BI, BJ, NX, NY, SCALED, FORM) <= 160 * 1024, "rings do not fit in LDS");
     constexpr bool HALVES = NY == 2, SPLIT = HALVES && NX == 3;
-    static_assert(SPLIT ? !SCALED && !SUM : NX == NY, "slots");
+    static_assert((SPLIT ? !SCALED && !SUM : NX == NY) && !(HALVES && SHORT), "slots");
     constexpr int XSW = BI / 128, YSW = BJ / 32;  // wavefronts' loads that a slot's scales take
     constexpr bool SHARED_SCALES = XSW + YSW <= 8;
-    constexpr int NLX = BI / 64, NLY = BJ / 64, EXTRA = SCALED ? (SHARED_SCALES ? 1 : 2) : SUM ? 1 : 0;
+    constexpr int NLX = BI / LOAD_I, NLY = BJ / LOAD_I, EXTRA = SCALED ? (SHARED_SCALES ? 1 : 2) : SUM ? 1 : 0;
     constexpr int LPAIR = NLX + NLY + EXTRA;  // loads a thread and slot
-    constexpr int NFRAG = (HALVES ? 1 : 2) * (TI + TJ);  // of a cluster
-    static_assert(BI % 128 == 0 && BJ % 64 == 0 && WTI % 32 == 0 && WTJ % 16 == 0, "tile");
+    constexpr int NFRAG = (HALVES || SHORT ? 1 : 2) * (TI + TJ);  // of a cluster
+    static_assert(BI % 128 == 0 && BJ % LOAD_I == 0 && WTI % 32 == 0 && WTJ % 16 == 0, "tile");
 
     extern __shared__ __attribute__((aligned(128))) char smem[];
     MIW_LDS char *lds = (MIW_LDS char *)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave % WI, wj = wave / WI, q = lane >> 4, r = lane & 15;
     const bool late_group = wave >= 4;
-    const int line = tid >> 3;  // this thread's row (k) of a load
+    // This thread's row (k) of a load; with slots of 32 a load takes two times 64 along i.
+    auto line_of = [](int t) MIW_INLINE { return SHORT ? (t >> 3) & 31 : t >> 3; };
+    const int line = line_of(tid);
     // Between tiles the arguments are read again and what hangs on the thread's number is made again: kept through the K loop
     // they would take more registers than there are.
     auto arguments = [] MIW_INLINE {
@@ -149,7 +181,7 @@ void k_grouped_tile(grouped_params p)
     auto find = [&](int workgroup) MIW_INLINE {
         walked_tile t;
         const auto a = arguments();
-        const int me = thread(), line = me >> 3;
+        const int me = thread(), line = line_of(me);
         grouped_tile at;
         if constexpr (SUM) at = find_sum_tile(*a, BI, BJ, workgroup);
         else at = find_tile(*a, BI, BJ, workgroup);
@@ -160,7 +192,7 @@ void k_grouped_tile(grouped_params p)
         for (int i = 0; i < ROWS; i++) t.rows[i] = 0;
         if (t.at.group >= 0 && t.at.first < t.at.last) {
 #pragma unroll
-            for (int i = 0; i < ROWS; i++) t.rows[i] = source_row(*a, min((YK ? t.at.j0 : t.at.first) + line + 64 * i, t.at.last - 1));
+            for (int i = 0; i < ROWS; i++) t.rows[i] = source_row(*a, min((YK ? t.at.j0 : t.at.first) + line + (SHORT ? 32 : 64) * i, t.at.last - 1));
             if constexpr (SCALED) t.scale_row = source_row(*a, min(t.at.j0 + 32 * y_part + ((me & 63) >> 1), t.at.last - 1));
         }
         return t;
@@ -183,7 +215,7 @@ void k_grouped_tile(grouped_params p)
     long xrow = 0, yrow = 0;     // (ragged sum: the lane's rows of the slot, in bytes from the operands)
     auto x_last_begins = [&]() MIW_INLINE {
         if constexpr (SUM) return;
-        const int me = thread(), line = me >> 3, k_chunk = k_chunk_of(me);
+        const int me = thread(), line = line_of(me), k_chunk = k_chunk_of(me);
         const unsigned back = XK ? 16u * (unsigned)max(0, k_chunk - (last_chunks - 1)) : (unsigned)(max(0, line - (last_values - 1)) * (int)p.ldx);
 #pragma unroll
         for (int i = 0; i < NLX; i++) xvo[i] -= back;
@@ -197,7 +229,7 @@ void k_grouped_tile(grouped_params p)
     };
     // Ragged sum: where this lane's row of slot `ynext` lies in both operands.
     auto find_rows = [&](int gathered) MIW_INLINE {
-        const int position = max(min(at.first + ynext * 64 + line, at.last - 1), 0);
+        const int position = max(min(at.first + ynext * SLOT_K + line, at.last - 1), 0);
         yrow = (long)position * p.ldy;
         xrow = (long)gathered * p.ldx;
     };
@@ -219,7 +251,7 @@ void k_grouped_tile(grouped_params p)
             else lds_load4<XRING + YBYTES>(ysp, lds0 + ywoff + (unsigned)y_part * 256u);
         } else if constexpr (SUM) {
             // the rows of the slot NY - 1 further on, by every wavefront to the same place
-            const int position = max(min(at.first + min(ynext + NY - 1, NP - 1) * 64 + lane, at.last - 1), 0);
+            const int position = max(min(at.first + min(ynext + NY - 1, NP - 1) * SLOT_K + lane, at.last - 1), 0);
             lds_load4<INDEX>((const char *)(p.gather ? p.gather + position : p.offsets), lds0 + index_entry(ynext + NY - 1));
         }
     };
@@ -254,11 +286,11 @@ void k_grouped_tile(grouped_params p)
     // nobody reads, and one of no rows for the row before).  The rings are empty then, and start at their beginnings.
     auto start = [&](const walked_tile &t) MIW_INLINE {
         const auto a = arguments();
-        const int me = thread(), line = me >> 3, k_chunk = k_chunk_of(me), i_chunk = i_chunk_of(me);
+        const int me = thread(), line = line_of(me), k_chunk = k_chunk_of(me), i_offset = 8 * i_chunk_of(me) + (SHORT ? 64 * (me >> 8) : 0);
         at = t.at;
         length = SUM ? at.last - at.first : a->K;
-        NP = (length + OP::slot_k - 1) / OP::slot_k;
-        last_values = length - (NP - 1) * OP::slot_k;
+        NP = (length + SLOT_K - 1) / SLOT_K;
+        last_values = length - (NP - 1) * SLOT_K;
         last_chunks = SCALED ? (last_values + 31) / 32 : (last_values + 7) / 8;
         xnext = ynext = 0;
         xwoff = ywoff = 0;
@@ -270,12 +302,12 @@ void k_grouped_tile(grouped_params p)
         } else {
             X += 2l * at.i0;
 #pragma unroll
-            for (int i = 0; i < NLX; i++) xvo[i] = (SUM ? 0u : (unsigned)(line * (int)a->ldx)) + 2u * (unsigned)min(64 * i + i_chunk * 8, a->I - 8 - at.i0);
+            for (int i = 0; i < NLX; i++) xvo[i] = (SUM ? 0u : (unsigned)(line * (int)a->ldx)) + 2u * (unsigned)min(LOAD_I * i + i_offset, a->I - 8 - at.i0);
         }
 #pragma unroll
         for (int i = 0; i < NLY; i++) {
             if constexpr (YK) yp[i] = a->Y + (long)t.rows[i] * a->ldy + k_chunk * 16;
-            else yp[i] = a->Y + 2l * (at.j0 + min(64 * i + i_chunk * 8, a->J - 8 - at.j0));
+            else yp[i] = a->Y + 2l * (at.j0 + min(LOAD_I * i + i_offset, a->J - 8 - at.j0));
         }
         if constexpr (SCALED) {
             xsp = (const char *)a->xs + (long)at.group * a->sxs + 8l * min((long)at.i0 + x_part * 128 + 2 * (me & 63), a->lxs - 2);
@@ -301,8 +333,8 @@ void k_grouped_tile(grouped_params p)
         }
     };
 
-    frag_reader<BI, XK> xr;
-    frag_reader<BJ, YK> yr;
+    std::conditional_t<SHORT, short_reader, frag_reader<BI, XK>> xr;
+    std::conditional_t<SHORT, short_reader, frag_reader<BJ, YK>> yr;
     xr.init(wi * WTI, lane);
     yr.init(wj * WTJ, lane);
     f32x4 acc[TI][TJ];
@@ -355,7 +387,7 @@ void k_grouped_tile(grouped_params p)
 #pragma unroll
         for (int b = 0; b < TJ; b++) acc[a][b] = f32x4{zero, zero, zero, zero};
     if (NP > 0) {
-        constexpr int FSETS = HALVES ? 1 : 2;
+        constexpr int FSETS = HALVES || SHORT ? 1 : 2;
         u32x4 fx[FSETS][TI], fy[FSETS][TJ];
         unsigned lane_sx[SCALED ? TI : 1], lane_sy[SCALED ? TJ : 1];  // this lane's scales of steps 0 and 1 in the low bytes
         const unsigned own_bytes = (unsigned)(q | (4 + q) << 8 | 0x0c0c0000);
@@ -375,7 +407,7 @@ void k_grouped_tile(grouped_params p)
             MIW_LDS const char *xs = lds + xroff, *ys = lds + XRING + yroff;
             if constexpr (SUM && Y_HERE) {
                 const int row = p.gather ? min(max(*(MIW_LDS const int *)(lds + INDEX + index_entry(ynext) + 4 * line), 0), p.source_rows - 1)
-                                         : min(at.first + ynext * 64 + line, at.last - 1);
+                                         : min(at.first + ynext * SLOT_K + line, at.last - 1);
                 find_rows(row);
             }
             u32x2 sx[SCALED ? TI : 1], sy[SCALED ? TJ : 1];  // a row's eight scales of the slot
@@ -467,10 +499,10 @@ void k_grouped_tile(grouped_params p)
                 wait_loads_and_barrier<INFLIGHT>();
                 if constexpr (MASK) {
                     mask_tail(step0, step0);
-                    mask_tail(step1, step1);
+                    if constexpr (!SHORT) mask_tail(step1, step1);
                 }
                 multiply(step0, step0);
-                multiply(step1, step1);
+                if constexpr (!SHORT) multiply(step1, step1);
             }
             __builtin_amdgcn_s_barrier();
         };

@@ -14,7 +14,7 @@ static hipError_t launch_tile_instance(grouped_params p, hipStream_t s)
     const void *fn = (const void *)k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>;
     static const hipError_t allowed = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (allowed != hipSuccess) return allowed;
-    const long blocks = FORM == RAGGED_SUM ? ((long)p.groups * ((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ) + 7) / 8 * 8 : grouped_blocks(p, BI, BJ, 512);
+    const long blocks = grouped_sums(FORM) ? ((long)p.groups * ((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ) + 7) / 8 * 8 : grouped_blocks(p, BI, BJ, 512);
     if (blocks <= 0 || blocks >= 1l << 23) return hipErrorInvalidConfiguration;
     p.most_tiles = (int)blocks;
     // Workgroups that walk their tiles request the next one's first slots ahead of the stores (16384 rows, 8 groups, 4096 x 4096, bf16:
@@ -29,8 +29,12 @@ static hipError_t launch_tile_size(const grouped_params &p, grouped_tile_size t,
 {
     switch (t) {
     case TILE_256x256: return launch_tile_instance<OP, 256, 256, 2, 4, OP::scaled || FORM == RAGGED_SUM ? 2 : 3, 2, FORM, DT>(p, s);
-    case TILE_256x128: return launch_tile_instance<OP, 256, 128, 4, 2, 3, 3, FORM, DT>(p, s);
-    case TILE_128x128: return launch_tile_instance<OP, 128, 128, 4, 2, FORM == RAGGED_SUM ? 2 : 4, FORM == RAGGED_SUM ? 2 : 4, FORM, DT>(p, s);
+    case TILE_256x128:
+        if constexpr (FORM == RAGGED_SUM) return launch_tile_instance<OP, 256, 128, 4, 2, 3, 3, RAGGED_SUM_32, DT>(p, s);
+        else return launch_tile_instance<OP, 256, 128, 4, 2, 3, 3, FORM, DT>(p, s);
+    case TILE_128x128:
+        if constexpr (FORM == RAGGED_SUM) return launch_tile_instance<OP, 128, 128, 4, 2, 2, 2, RAGGED_SUM, DT>(p, s);
+        else return launch_tile_instance<OP, 128, 128, 4, 2, 4, 4, FORM, DT>(p, s);
     default: return launch_tile_instance<OP, 128, 64, 4, 2, 6, 6, FORM, DT>(p, s);
     }
 }

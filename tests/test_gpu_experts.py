@@ -321,6 +321,12 @@ def test_grouped_wgrad_large(gpu, rows, groups, m, n, kind, out):
         assert np.array_equal(D.to_host().reshape(groups, m, n), 2 * want)
 
 
+@pytest.mark.parametrize("rows,groups,m,n,kind,out", [(1601, 1, 3496, 3592, "bf16", "f32"), (4703, 3, 2056, 1992, "f16", "f16"), (1537, 1, 3592, 3496, "f16", "f32")])
+def test_grouped_wgrad_large_and_long(gpu, rows, groups, m, n, kind, out):
+    """Sums so long that the largest tile takes them (with an empty group among three)."""
+    test_grouped_wgrad_large(gpu, rows, groups, m, n, kind, out)
+
+
 def test_grouped_gemm_offsets_and_gather_outside(gpu):
     """Offsets and rows that lie outside are taken as the nearest inside: nothing else is read or written."""
     rng = np.random.default_rng(1)
