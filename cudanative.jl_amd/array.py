@@ -75,6 +75,10 @@ class DevicePtr:
     def __int__(self):
         return self.addr
 
+    @property
+    def _as_parameter_(self):
+        return self.addr
+
     def __repr__(self):
         return f"DevicePtr{{{self.eltype.name},{self.addrspace}}}(0x{self.addr:016x})"
 
@@ -128,6 +132,11 @@ class DeviceArray:
     @property
     def shape(self):
         return self.dims
+
+    @property
+    def _as_parameter_(self):
+        """What ctypes passes for the array: its address."""
+        return self.ptr
 
     def __len__(self):
         return int(np.prod(self.dims, dtype=np.int64))

@@ -217,3 +217,19 @@ def test_gated_silu_refusals(miw):
     refused(L.ERR_INVALID_VALUE, E.gated_silu_grad, P, 2 * P, 3 * P, **ok, ldda=3)
     refused(L.ERR_INVALID_VALUE, E.gated_silu_grad, P, 2 * P, 3 * P, **ok, lddz=7)
     refused(L.ERR_INVALID_VALUE, E.gated_silu_grad, P, 2 * P, P, **ok, ldz=8, lddz=16)
+
+
+def test_addresses_that_are_no_plain_integers(miw):
+    """numpy's integers and typed pointers are addresses too; other numbers are not.  (Nothing is launched for no rows, and a
+    null address is looked at first.)"""
+    E, L = miw.EXPERTS, miw._lib
+    E.gated_silu(np.int64(1 << 20), np.uint64(1 << 21), rows=0, n=8)
+    null, typed = miw.DevicePtr(np.float16, 0), miw.DevicePtr(np.float16, 1 << 20)
+    for Z, A in ((null, typed), (typed, null), (np.int64(0), typed)):
+        with pytest.raises(miw.MIWError) as e:
+            E.gated_silu(Z, A, rows=4, n=8)
+        assert e.value.code == L.ERR_NULL_POINTER
+    with pytest.raises(TypeError):
+        E.gated_silu(1.5, 1 << 20, rows=4, n=8)
+    with pytest.raises(TypeError):
+        E.gated_silu("a", 1 << 20, rows=4, n=8, dtype="no type")
