@@ -2,7 +2,7 @@
 //
 // Choice.  A lane holds logits as unsigned keys in the order of the values (0: never chosen).  Up to 256 experts a token has sixteen
 // lanes, four tokens a wavefront: the largest key and the lowest expert that has it are two reductions over a row of lanes by
-// data-parallel moves, so equal logits go to the lowest expert.  What bounds it is the number of instructions: with a wavefront for every
+// data-parallel moves, so equal logits go to the lowest expert; 16-bit logits carry the expert in the key's low half, and one reduction does.  What bounds it is the number of instructions: with a wavefront for every
 // token, forty of them a choice in place of fourteen, the first launch of the case below took 12.4 us.  Beyond 256 experts a token has a
 // wavefront, and a ballot per register finds the expert.
 // Order.  Counting sort in two launches over at most 256 chunks of tokens (one launch for up to 64 tokens).  The first counts its chunk's
@@ -11,7 +11,7 @@
 // lower experts and earlier chunks and writes the positions.  Counts are integers: no order of theirs matters.
 //
 // Bound by latency throughout: 16381 tokens, 128 experts, 8 choices (bf16): 4.2 MB of logits, 1.6 MB of results:
-// choose 8.7 us, place 8.3 us, gradient 5.9 us (8.4 MB in and out; with a wavefront a token 7.8) where the bytes alone take one to two each.  16 tokens of 64
+// choose 8.5 us (9.4 with two reductions), place 8.0 us, gradient 6.0 us (8.4 MB in and out; with a wavefront a token 7.8) where the bytes alone take one to two each.  16 tokens of 64
 // experts, 4 choices: one launch of 3.2 us.
 #include "experts.hpp"
 #include "vec_types.hpp"
@@ -37,6 +37,22 @@ __device__ inline unsigned order_key(float z)
 __device__ inline float key_value(unsigned key)
 {
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// Logits of 16 bits have keys of 16, and the expert fits beside them: the largest such number names the largest logit and, of equal ones,
+// the lowest expert, by one reduction.
+template <class T>
+__device__ inline unsigned packed_key(T z, int expert)
+{
+    const unsigned u = z == (T)0.f ? 0u : __builtin_bit_cast(unsigned short, z);
+    const unsigned key = u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+    return (float)z > -__builtin_inff() ? key << 16 | (0xffffu - (unsigned)expert) : 0u;
+}
+template <class T>
+__device__ inline float packed_value(unsigned packed)
+{
+    const unsigned key = packed >> 16;
+    return (float)__builtin_bit_cast(T, (unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
 }
 
 // Over the sixteen lanes of a row, to all of them; sums pair the same lanes in every lane.
@@ -73,11 +89,17 @@ __device__ inline void choose_row(const route_params &p, int base, int first, in
     const int lane = threadIdx.x & 15, token = first + ((threadIdx.x & 63) >> 4);
     const bool in = token < last;
     const T *z = (const T *)p.logits + (long)(in ? token : first) * p.ld;
+    constexpr bool PACKED = sizeof(T) == 2;
+    auto value_of = [](unsigned k) {
+        if constexpr (PACKED) return fminf(packed_value<T>(k), LARGEST);
+        else return fminf(key_value(k), LARGEST);
+    };
     unsigned key[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
         const int e = lane + 16 * i;
-        key[i] = e < p.experts ? order_key((float)z[e]) : 0u;
+        if constexpr (PACKED) key[i] = e < p.experts ? packed_key(z[e], e) : 0u;
+        else key[i] = e < p.experts ? order_key(z[e]) : 0u;
     }
     int mine = -1;  // lane j: choice j
     float value = 0.f, largest = 0.f, every = 0.f;
@@ -86,20 +108,27 @@ __device__ inline void choose_row(const route_params &p, int base, int first, in
 #pragma unroll
         for (int i = 1; i < R; i++) most = max(most, key[i]);
         most = row_max(most);
-        int expert = 1 << 30;
-#pragma unroll
-        for (int i = R - 1; i >= 0; i--) expert = key[i] == most ? lane + 16 * i : expert;
-        expert = row_min(expert);
-        const float v = fminf(key_value(most), LARGEST);
+        const float v = value_of(most);
         if (j == 0) {
             largest = v;
             if (p.over_all)
 #pragma unroll
-                for (int i = 0; i < R; i++) every += key[i] ? __expf(fminf(key_value(key[i]), LARGEST) - v) : 0.f;
+                for (int i = 0; i < R; i++) every += key[i] ? __expf(value_of(key[i]) - v) : 0.f;
         }
-        const int hit = (expert & 15) == lane ? expert >> 4 : -1;
+        int expert;
+        if constexpr (PACKED) {
+            expert = 0xffff - (int)(most & 0xffffu);
 #pragma unroll
-        for (int i = 0; i < R; i++) key[i] = hit == i ? 0u : key[i];
+            for (int i = 0; i < R; i++) key[i] = key[i] == most ? 0u : key[i];
+        } else {
+            expert = 1 << 30;
+#pragma unroll
+            for (int i = R - 1; i >= 0; i--) expert = key[i] == most ? lane + 16 * i : expert;
+            expert = row_min(expert);
+            const int hit = (expert & 15) == lane ? expert >> 4 : -1;
+#pragma unroll
+            for (int i = 0; i < R; i++) key[i] = hit == i ? 0u : key[i];
+        }
         if (lane == j && most) {
             mine = expert;
             value = v;
