@@ -64,17 +64,35 @@ static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int
     return best->size;
 }
 
-// A ragged sum writes every group's whole result, and the larger a tile the less often the operands are read: the largest one whose tiles fill
-// three quarters of the CUs.  Up to 1500 rows a group the tile's start and end count more than that, and 256 x 128 with slots of 32,
-// of which a CU holds two workgroups, comes first (16 groups, 2048 x 4096, Float32: 128 rows 142 us, 154 on 256 x 256; 512 rows 236 and 258;
-// but 8 groups of 2048 rows, 4096 x 4096: 618 and 560.  One group of 2048 rows, 1024 x 1024, 16 of the largest tiles: 47 us, 22 on 128 x 64).
+// Ragged sums, priced in the same way: a tile's start and end with its stores, and 64 rows of its sum, where a CU holds one workgroup (256 x 256,
+// 128 x 64) or two.  105 sums (1 to 128 groups, 304 to 4096 wide, 1 to 2048 rows a group): 1.01 of the fastest tile's time in the mean, 1.17 at worst.
+// 16 groups, 2048 x 4096, Float32: 128 rows 142 us on 256 x 128 with slots of 32, 154 on 256 x 256; 8 groups of 2048 rows, 4096 x 4096: 618 and
+// 560; 7 groups of 330 rows, 3040 x 336: 16.4 us on 128 x 128, 21.4 on 256 x 128; one group of 2048 rows, 1024 x 1024: 22 on 128 x 64, 30 on 128 x 128.
+struct sum_price {
+    grouped_tile_size size;
+    int bi, bj, together;
+    double tile, slot;
+};
+static const sum_price g_sums[] = {
+    {TILE_256x256, 256, 256, 1, 9.1, 1.40},
+    {TILE_256x128, 256, 128, 2, 6.6, 1.55},
+    {TILE_128x128, 128, 128, 2, 4.7, 0.88},
+    {TILE_128x64, 128, 64, 1, 4.7, 0.39},
+};
 static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
 {
-    for (const tile_price &t : g_tiles) {
-        if (t.size == TILE_256x256 && p.rows < 1500l * p.groups) continue;
-        if (p.groups * ceil_div(p.I, t.bi) * ceil_div(p.J, t.bj) >= 3l * cus / 4) return t.size;
+    const double slots = (double)p.rows / p.groups / 64 + (p.groups > 1 ? 0.5 : 0.0);
+    const sum_price *best = nullptr;
+    double best_us = 0.0;
+    for (const sum_price &t : g_sums) {
+        const double rounds = (double)p.groups * (double)ceil_div(p.I, t.bi) * (double)ceil_div(p.J, t.bj) / (t.together * cus);
+        const double us = (rounds >= 3 ? rounds + 0.25 : std::max(1.0, (double)(long)(rounds + 0.95))) * (t.tile + slots * t.slot);
+        if (!best || us < best_us) {
+            best = &t;
+            best_us = us;
+        }
     }
-    return TILE_128x64;
+    return best->size;
 }
 
 hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s)
