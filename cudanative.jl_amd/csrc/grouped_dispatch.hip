@@ -3,10 +3,11 @@
 // How many rows a group has is not known on the host: the rules go by the mean, rows / groups.  Their numbers come from some 400
 // products timed on every kernel (1 to 128 groups, 512 to 4096 wide, 0.5 to 2048 rows a group whose loads differ by up to three
 // times, f16 with k or i contiguous in the weights and 4 bits, weights from HBM): the rule's kernel takes 1.01 (f16) and 1.02 (4 bits)
-// of the fastest one's time in the geometric mean, at worst 1.38 (8 groups of 384 rows in the mean, whose real loads make whole rounds).
+// of the fastest one's time in the geometric mean, at worst 1.38 and 1.52 (loads that happen to make a round more or less).
 #include "experts.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace miw {
 
@@ -43,7 +44,8 @@ static const tile_price g_tiles[] = {
 };
 
 // Ragged rows: the tile with the shortest estimated launch, rounds of tiles over the CUs at the measured price of each.  A group's
-// last tile is half full in the mean.
+// last tile is half full in the mean, and off that by 0.29 of a tile (the root of 1/12): a round is counted where there are tiles for it beyond what
+// that makes of all groups together.
 static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int cus)
 {
     const double per_group = (double)p.rows / p.groups, slots = (double)ceil_div(p.K, slot_k);
@@ -52,7 +54,8 @@ static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int
     for (const tile_price &t : g_tiles) {
         const double high = p.groups == 1 ? (double)ceil_div(p.rows, t.bj) : per_group <= 0.5 * t.bj ? 1.0 : per_group / t.bj + 0.5;
         const double rounds = (double)std::min(p.groups, p.rows) * high * (double)ceil_div(p.I, t.bi) / cus;
-        const double whole = rounds >= 8 ? rounds + 0.5 : std::max(1.0, (double)(long)(rounds + 0.95));
+        const double spread = p.groups > 1 && per_group > 0.5 * t.bj ? std::sqrt(p.groups / 12.0) * (double)ceil_div(p.I, t.bi) / cus : 0.0;
+        const double whole = rounds >= 8 ? rounds + 0.5 : std::max(1.0, (double)(long)std::max(rounds + 0.995 - spread, 0.0));
         const double us = whole * (slot_k == 64 ? t.f16_tile + slots * t.f16_slot : t.mxfp4_tile + slots * t.mxfp4_slot);
         if (!best || us < best_us) {
             best = &t;
