@@ -2,7 +2,7 @@
 //
 // How many rows a group has is not known on the host: the rules go by the mean, rows / groups.  Their numbers come from some 400
 // products timed on every kernel (1 to 128 groups, 512 to 4096 wide, 0.5 to 2048 rows a group whose loads differ by up to three
-// times, f16 with k or i contiguous in the weights and 4 bits, weights from HBM): the rule's kernel takes 1.01 (f16) and 1.02 (4 bits)
+// times, f16 with k or i contiguous in the weights and 4 bits, weights from HBM): the rule's kernel takes 1.007 (f16) and 1.012 (4 bits)
 // of the fastest one's time in the geometric mean, at worst 1.38 and 1.52 (loads that happen to make a round more or less).
 #include "experts.hpp"
 
@@ -37,10 +37,10 @@ struct tile_price {
     double f16_slot, f16_tile, mxfp4_slot, mxfp4_tile;  // microseconds for a slot of k and for a tile's start and end
 };
 static const tile_price g_tiles[] = {
-    {TILE_256x256, 256, 256, 1.35, 6.4, 1.90, 6.5},
-    {TILE_256x128, 256, 128, 0.92, 3.6, 0.95, 4.6},
-    {TILE_128x128, 128, 128, 0.58, 6.3, 0.68, 4.0},
-    {TILE_128x64, 128, 64, 0.36, 3.3, 0.48, 2.9},
+    {TILE_256x256, 256, 256, 1.35, 6.4, 1.33, 12.0},
+    {TILE_256x128, 256, 128, 0.92, 3.6, 0.89, 7.2},
+    {TILE_128x128, 128, 128, 0.58, 6.3, 0.57, 6.0},
+    {TILE_128x64, 128, 64, 0.36, 3.3, 0.50, 4.4},
 };
 
 // Ragged rows: the tile with the shortest estimated launch, rounds of tiles over the CUs at the measured price of each.  A group's
