@@ -63,6 +63,14 @@ constexpr int grouped_lds_bytes(int bi, int bj, int nx, int ny, bool scaled, int
     return nx * grouped_slot_bytes(bi, scaled, form) + ny * grouped_slot_bytes(bj, scaled, form) + (grouped_sums(form) ? 2 * ny * 256 : 0);
 }
 
+// X's scales of a tile are fetched 16 bytes, two rows, a lane, 128 rows a wavefront's load: the first row, of the matrix' I, of such a
+// pair.  Rows behind the matrix' last pair repeat it: panels may hold other matrices' rows there, or end.
+constexpr int scale_pair(int i0, int part, int lane, int I)
+{
+    const int row = i0 + part * 128 + 2 * lane, last = I + (I & 1) - 2;
+    return row < last ? row : last;
+}
+
 // Workgroups that a CU holds together.
 constexpr int grouped_workgroups(int bi, int bj, int nx, int ny, bool scaled, int form)
 {
@@ -316,7 +324,7 @@ void k_grouped_tile(grouped_params p)
             else yp[i] = a->Y + 2l * (at.j0 + min(LOAD_I * i + i_offset, a->J - 8 - at.j0));
         }
         if constexpr (SCALED) {
-            xsp = (const char *)a->xs + (long)at.group * a->sxs + 8l * min((long)at.i0 + x_part * 128 + 2 * (me & 63), a->lxs - 2);
+            xsp = (const char *)a->xs + (long)at.group * a->sxs + 8l * scale_pair(at.i0, x_part, me & 63, a->I);
             ysp = (const char *)a->ys + 8l * t.scale_row + 4 * (me & 1);
         }
         if (NP == 1) {

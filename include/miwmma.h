@@ -408,7 +408,9 @@ int miw_combine_grad(int dtype, int64_t tokens, int top, int64_t n, int64_t rows
              16 * ceil(k / 32), on 16-byte addresses.  What a last block has beyond k is written as zeros.
      scales  in panels of eight blocks: byte ((p * lds + r) * 8 + b) is the scale of row r's block 8 p + b, for
              ceil(k / 256) panels of lds rows (an even number of at least `rows`), on 16-byte addresses.
-   Pitches of 0: dense (16 * ceil(k / 32) bytes; rows rounded up to an even number). */
+   Pitches of 0: dense (16 * ceil(k / 32) bytes; rows rounded up to an even number).
+   Panels may be shared: matrices whose rows lie one behind the other, each on an even row, are one tall matrix with one lds, and
+   a product reads of each panel only its matrix' own rows, up to an even number. */
 
 /* A block's scale is 2^(floor(log2(its largest magnitude)) - 2), kept in -127 .. 127; its values are divided by that,
    rounded to the nearest (ties to the even code) and kept within 6.  A block of zeros has scale 0 (2^-127); one that holds an

@@ -1,0 +1,53 @@
+"""Functions of the grouped products' kernels and dispatch that also run on the host: addresses and choices of kernels, without a GPU."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+SCALES = """
+#include "grouped_tile.hpp"
+#include <cstdio>
+// Matrices of n rows each, one behind the other in each panel of lds rows of scales (the last one's rows end where the panel ends, or `more`
+// rows before that): the bytes that a tile's loads of scales touch in the last panel of the last matrix.
+int main()
+{
+    for (long n : {1l, 2l, 38l, 130l, 192l, 1087l, 1088l, 2879l, 2880l})
+        for (long matrices : {1l, 2l, 5l})
+            for (long more : {0l, 2l, 300l})
+                for (int bi : {128, 256}) {
+                    const long own = n + n % 2, lds = matrices * own + more, base = (matrices - 1) * own;
+                    for (long i0 = 0; i0 < n; i0 += bi)
+                        for (int part = 0; part < bi / 128; part++)
+                            for (int lane = 0; lane < 64; lane++) {
+                                const long row = miw::scale_pair((int)i0, part, lane, (int)n), wanted = i0 + 128 * part + 2 * lane;
+                                if (row < 0 || row % 2 || base + row + 2 > matrices * own || (wanted < n && row != wanted)) {
+                                    std::printf("%ld matrices of %ld rows, panels of %ld, tile of %d at %ld: part %d, lane %d reads rows %ld and %ld", matrices, n, lds, bi, i0, part, lane,
+                                                base + row, base + row + 1);
+                                    return 1;
+                                }
+                            }
+                }
+    return 0;
+}
+"""
+
+
+def _run(tmp_path, source):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    src, exe = tmp_path / "host.hip", tmp_path / "host"
+    src.write_text(source)
+    r = subprocess.run([hipcc, "--offload-arch=gfx950", "-O1", "-std=c++20", "-Wno-inline-asm", "-I" + os.path.join(ROOT, "cudanative.jl_amd", "csrc"),
+                        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", str(src), "-o", str(exe)], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-2000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+
+
+def test_loads_of_scales_stay_inside_their_matrix(tmp_path):
+    """4-bit matrices that lie one behind the other in panels: no load of the last one's scales goes beyond its rows."""
+    _run(tmp_path, SCALES)
