@@ -111,7 +111,7 @@ int miw_route_workspace(int64_t tokens, int experts, int top, size_t *bytes)
 {
     if (!bytes) return api_fail(MIW_ERR_NULL_POINTER, "route_workspace: null output pointer");
     CHECK(check_routing("route_workspace", MIW_F32, tokens, experts, top));
-    const int chunks = miw::route_chunks(tokens);
+    const int chunks = miw::route_most_chunks(tokens);
     *bytes = chunks == 1 ? 0 : (size_t)chunks * (size_t)experts * sizeof(int);
     return 0;
 }

@@ -24,8 +24,8 @@ struct route_params {
     long ld;
     int chunks, chunk;  // chunks of `chunk` tokens
 };
-// Chunks that the tokens are cut into; 1: one workgroup does everything and there is no workspace.
-int route_chunks(long tokens);
+// The most chunks that up to so many tokens are cut into; 1: one workgroup does everything and there is no workspace.
+int route_most_chunks(long tokens);
 hipError_t launch_route(route_params p, int dtype, hipStream_t s);
 struct route_grad_params {
     const void *logits;

@@ -387,12 +387,19 @@ __global__ __launch_bounds__(256) void k_route_grad(route_grad_params p)
 }
 
 // At most 256 chunks of sixteen tokens (one a wavefront) or more; one workgroup as long as it has its tokens together.
+constexpr int ROUTE_CHUNKS = 256;
 static int route_chunk(long tokens)
 {
-    const long chunk = (tokens + 255) / 256;
+    const long chunk = (tokens + ROUTE_CHUNKS - 1) / ROUTE_CHUNKS;
     return (int)(chunk < ROUTE_WAVES ? ROUTE_WAVES : chunk);
 }
-int route_chunks(long tokens)
+// (The number of chunks falls where the chunk becomes a token longer.)
+int route_most_chunks(long tokens)
+{
+    const long chunks = (tokens + ROUTE_WAVES - 1) / ROUTE_WAVES;
+    return tokens <= ROUTE_TOKENS ? 1 : (int)(chunks < ROUTE_CHUNKS ? chunks : ROUTE_CHUNKS);
+}
+static int route_chunks(long tokens)
 {
     return tokens <= ROUTE_TOKENS ? 1 : (int)((tokens + route_chunk(tokens) - 1) / route_chunk(tokens));
 }

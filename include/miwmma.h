@@ -360,7 +360,7 @@ int miw_copy_probe(void *dst, const void *src, size_t bytes, void *stream);
      rows   [tokens * top]   token at each sorted position (by expert, then by token); -1 from offsets[experts] on
      place  [tokens x top]   sorted position of each choice, or -1
    At most 1024 experts, top of at most 16 and of `experts`, tokens * top at most 2^30.  The workspace (miw_route_workspace bytes, 16-byte
-   aligned; 0 bytes: it may be null) needs no clearing.  The same bits every time. */
+   aligned; 0 bytes: it may be null) needs no clearing; one for some number of tokens and experts suffices for fewer.  The same bits every time. */
 int miw_route_workspace(int64_t tokens, int experts, int top, size_t *bytes);
 int miw_route(int dtype, int64_t tokens, int experts, int top, int64_t ld, int over_all, const void *logits, int *chosen,
               float *gates, int *offsets, int *rows, int *place, void *workspace, size_t workspace_bytes, void *stream);

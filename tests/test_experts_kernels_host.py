@@ -51,3 +51,11 @@ def _run(tmp_path, source):
 def test_loads_of_scales_stay_inside_their_matrix(tmp_path):
     """4-bit matrices that lie one behind the other in panels: no load of the last one's scales goes beyond its rows."""
     _run(tmp_path, SCALES)
+
+
+@pytest.mark.parametrize("experts", [1, 16, 1024])
+def test_route_workspace_never_falls_as_tokens_grow(miw, experts):
+    """What suffices for the most tokens of a program suffices for all its calls."""
+    need = [miw.EXPERTS.route_workspace(t, experts, 1) for t in [*range(0, 20000), *(1 << b for b in range(15, 31))]]
+    assert not any(need[:65]) and need[65] > 0
+    assert all(a <= b for a, b in zip(need, need[1:]))
