@@ -106,7 +106,27 @@ struct grouped_narrow_form {
 hipError_t launch_grouped_narrow(const grouped_params &p, grouped_narrow_form f, int dtype, int d_type, hipStream_t s);
 hipError_t launch_grouped_mxfp4_narrow(const grouped_params &p, grouped_narrow_form f, int d_type, hipStream_t s);
 // --- grouped_dispatch.hip: the kernel that runs a product.
+enum grouped_kernel { GROUPED_PLAIN, GROUPED_NARROW, GROUPED_TILE };
+struct grouped_choice {
+    int kernel;
+    grouped_narrow_form narrow;  // GROUPED_NARROW
+    int tile;                    // GROUPED_TILE
+    long workgroups;             // that it asks for, or tiles where workgroups walk them (not set for GROUPED_PLAIN)
+};
+grouped_choice choose_grouped(const grouped_params &p, bool mxfp4, bool ragged_sum, int cus);
 hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s);
 hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, int cus, hipStream_t s);
+
+// Workgroups of a launch over tiles of bi x bj: at most ceil(rows / bj) and one more for each group, or the sums' own number; whole eighths, since
+// an XCD's share may be one more than that.
+inline long grouped_blocks(const grouped_params &p, long bi, long bj, bool ragged_sum)
+{
+    const long tiles_i = (p.I + bi - 1) / bi;
+    const long tiles_j = ragged_sum ? (long)p.groups * ((p.J + bj - 1) / bj) : p.rows / bj + (p.groups < p.rows ? p.groups : p.rows);
+    return (tiles_i * tiles_j + 7) / 8 * 8;
+}
+// A launch has fewer than 2^32 threads; tiles that workgroups walk are counted in an int.
+constexpr bool grid_fits(long workgroups, long threads) { return workgroups < (1l << 32) / threads; }
+constexpr long MOST_WALKED_TILES = 1l << 30;
 
 }  // namespace miw

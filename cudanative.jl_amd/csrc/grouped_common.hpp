@@ -85,15 +85,6 @@ __device__ inline grouped_tile find_tile(const PARAMS &p, int bi, int bj, int wo
     return {g0 + at, __builtin_amdgcn_readfirstlane(rows.first), __builtin_amdgcn_readfirstlane(rows.last),
             __builtin_amdgcn_readfirstlane(rows.first) + j * bj, i * bi};
 }
-// Workgroups of a launch over tiles of bi x bj, or 0 where they do not fit in a grid.
-inline long grouped_blocks(const grouped_params &p, long bi, long bj, long threads)
-{
-    const long tiles = (p.rows / bj + (p.groups < p.rows ? p.groups : p.rows)) * ((p.I + bi - 1) / bi);
-    const long n = (tiles + 7) / 8 * 8;  // (an XCD's share may be one more than a whole number of eighths)
-    return n * threads < (1l << 32) && n < (1l << 30) ? n : 0;
-}
-
-
 // Stores the four results i .. i + 3 of row j; those from I on are left out.  In the gated form they are two pairs of gate and
 // value, and two results are stored (I counts the columns before that).
 template <class DT, class PARAMS>

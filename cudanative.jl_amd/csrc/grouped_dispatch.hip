@@ -28,7 +28,9 @@ static grouped_narrow_form pick_narrow(const grouped_params &p, int slot_k)
     if (workgroups <= 256 && per_group <= 64) return {per_group <= 16 ? 1 : per_group <= 32 ? 2 : 4, 1, 8};
     if (per_group > 10) return {0, 0, 0};
     if (chunks >= 64 && workgroups <= 1024) return {1, 1, 8};
-    return {1, 2, chunks >= 16 ? 4 : 2};
+    const int waves = chunks >= 16 ? 4 : 2;
+    if (!grid_fits(workgroups, 64 * waves)) return {0, 0, 0};  // (it has a workgroup for every group, with rows or without; a tile's launch has not)
+    return {1, 2, waves};
 }
 
 struct tile_price {
@@ -52,6 +54,7 @@ static grouped_tile_size pick_rows_tile(const grouped_params &p, int slot_k, int
     const tile_price *best = nullptr;
     double best_us = 0.0;
     for (const tile_price &t : g_tiles) {
+        if (best && slot_k == 256 && !grid_fits(grouped_blocks(p, t.bi, t.bj, false), 512)) continue;  // (4 bits: no walk)
         const double high = p.groups == 1 ? (double)ceil_div(p.rows, t.bj) : per_group <= 0.5 * t.bj ? 1.0 : per_group / t.bj + 0.5;
         const double rounds = (double)std::min(p.groups, p.rows) * high * (double)ceil_div(p.I, t.bi) / cus;
         const double spread = p.groups > 1 && per_group > 0.5 * t.bj ? std::sqrt(p.groups / 12.0) * (double)ceil_div(p.I, t.bi) / cus : 0.0;
@@ -88,6 +91,7 @@ static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
     const sum_price *best = nullptr;
     double best_us = 0.0;
     for (const sum_price &t : g_sums) {
+        if (best && !grid_fits(grouped_blocks(p, t.bi, t.bj, true), 512)) continue;
         const double rounds = (double)p.groups * (double)ceil_div(p.I, t.bi) * (double)ceil_div(p.J, t.bj) / (t.together * cus);
         const double us = (rounds >= 3 ? rounds + 0.25 : std::max(1.0, (double)(long)(rounds + 0.95))) * (t.tile + slots * t.slot);
         if (!best || us < best_us) {
@@ -98,21 +102,32 @@ static grouped_tile_size pick_sum_tile(const grouped_params &p, int cus)
     return best->size;
 }
 
-hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s)
+grouped_choice choose_grouped(const grouped_params &p, bool mxfp4, bool ragged_sum, int cus)
 {
     // (lane offsets of 256 rows, or of 64 along k, are 32 bits; a sum over no rows has none to fetch)
-    if (!p.vector || 256 * p.ldx >= 1l << 31 || p.rows == 0) return launch_grouped_plain(p, dtype, d_type, ragged_sum, s);
+    if (!p.vector || 256 * p.ldx >= 1l << 31 || p.rows == 0) return {GROUPED_PLAIN, {0, 0, 0}, 0, 0};
+    const int slot_k = mxfp4 ? 256 : 64;
     if (!ragged_sum)
-        if (const grouped_narrow_form f = pick_narrow(p, 64); f.mt) return launch_grouped_narrow(p, f, dtype, d_type, s);
-    const grouped_tile_size t = ragged_sum ? pick_sum_tile(p, cus) : pick_rows_tile(p, 64, cus);
-    return (dtype == TYPE_F16 ? launch_grouped_tile_f16 : launch_grouped_tile_bf16)(p, t, d_type, ragged_sum, s);
+        if (const grouped_narrow_form f = pick_narrow(p, slot_k); f.mt) return {GROUPED_NARROW, f, 0, p.groups * ceil_div(p.I, 16 * f.wt)};
+    const grouped_tile_size size = ragged_sum ? pick_sum_tile(p, cus) : pick_rows_tile(p, slot_k, cus);
+    const tile_price &t = *std::find_if(std::begin(g_tiles), std::end(g_tiles), [&](const tile_price &x) { return x.size == size; });
+    return {GROUPED_TILE, {0, 0, 0}, size, grouped_blocks(p, t.bi, t.bj, ragged_sum)};
+}
+
+hipError_t launch_grouped(const grouped_params &p, int dtype, int d_type, bool ragged_sum, int cus, hipStream_t s)
+{
+    const grouped_choice c = choose_grouped(p, false, ragged_sum, cus);
+    if (c.kernel == GROUPED_PLAIN) return launch_grouped_plain(p, dtype, d_type, ragged_sum, s);
+    if (c.kernel == GROUPED_NARROW) return launch_grouped_narrow(p, c.narrow, dtype, d_type, s);
+    return (dtype == TYPE_F16 ? launch_grouped_tile_f16 : launch_grouped_tile_bf16)(p, (grouped_tile_size)c.tile, d_type, ragged_sum, s);
 }
 
 hipError_t launch_grouped_mxfp4(const grouped_params &p, int d_type, int cus, hipStream_t s)
 {
-    if (256 * p.ldx >= 1l << 31) return launch_grouped_mxfp4_plain(p, d_type, s);
-    if (const grouped_narrow_form f = pick_narrow(p, 256); f.mt) return launch_grouped_mxfp4_narrow(p, f, d_type, s);
-    return launch_grouped_tile_mxfp4(p, pick_rows_tile(p, 256, cus), d_type, s);
+    const grouped_choice c = choose_grouped(p, true, false, cus);
+    if (c.kernel == GROUPED_PLAIN) return launch_grouped_mxfp4_plain(p, d_type, s);
+    if (c.kernel == GROUPED_NARROW) return launch_grouped_mxfp4_narrow(p, c.narrow, d_type, s);
+    return launch_grouped_tile_mxfp4(p, (grouped_tile_size)c.tile, d_type, s);
 }
 
 }  // namespace miw

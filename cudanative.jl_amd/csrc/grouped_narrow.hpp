@@ -154,7 +154,6 @@ template <class OP, class DT>
 static hipError_t launch_narrow_type(const grouped_params &p, grouped_narrow_form f, hipStream_t s)
 {
     const long blocks = (long)p.groups * ((p.I + 16 * f.wt - 1) / (16 * f.wt));
-    if (blocks >= 1l << 22) return hipErrorInvalidConfiguration;
     auto with_rows = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         if (f.wt == 1) hipLaunchKernelGGL((k_grouped_narrow<OP, MT, 1, 8, 2, DT>), dim3((unsigned)blocks), dim3(512), 0, s, p);

@@ -114,8 +114,8 @@ __global__ __launch_bounds__(256) void k_grouped_plain(grouped_params p)
 
 hipError_t launch_grouped_plain(grouped_params p, int dtype, int d_type, bool ragged_sum, hipStream_t s)
 {
-    const long blocks = ragged_sum ? (long)p.groups * ((p.I + PLAIN - 1) / PLAIN) * ((p.J + PLAIN - 1) / PLAIN) : grouped_blocks(p, PLAIN, PLAIN, 256);
-    if (blocks <= 0 || blocks >= 1l << 24) return hipErrorInvalidConfiguration;
+    const long blocks = ragged_sum ? (long)p.groups * ((p.I + PLAIN - 1) / PLAIN) * ((p.J + PLAIN - 1) / PLAIN) : grouped_blocks(p, PLAIN, PLAIN, false);
+    if (!grid_fits(blocks, 256)) return hipErrorInvalidConfiguration;
     p.most_tiles = (int)blocks;
     const dim3 grid((unsigned)blocks), block(256);
     auto go = [&](auto mfma, auto type) {
@@ -160,8 +160,8 @@ __global__ __launch_bounds__(64) void k_grouped_mxfp4_plain(grouped_params p)
 
 hipError_t launch_grouped_mxfp4_plain(grouped_params p, int d_type, hipStream_t s)
 {
-    const long blocks = grouped_blocks(p, 16, 16, 64);
-    if (blocks <= 0) return hipErrorInvalidConfiguration;
+    const long blocks = grouped_blocks(p, 16, 16, false);
+    if (!grid_fits(blocks, 64)) return hipErrorInvalidConfiguration;
     p.most_tiles = (int)blocks;
     const dim3 grid((unsigned)blocks), block(64);
     if (d_type == TYPE_F32) hipLaunchKernelGGL(k_grouped_mxfp4_plain<float>, grid, block, 0, s, p);

@@ -14,13 +14,14 @@ static hipError_t launch_tile_instance(grouped_params p, hipStream_t s)
     const void *fn = (const void *)k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>;
     static const hipError_t allowed = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (allowed != hipSuccess) return allowed;
-    const long blocks = grouped_sums(FORM) ? ((long)p.groups * ((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ) + 7) / 8 * 8 : grouped_blocks(p, BI, BJ, 512);
-    if (blocks <= 0 || blocks >= 1l << 23) return hipErrorInvalidConfiguration;
+    constexpr bool walks = grouped_walks(OP::scaled, FORM);
+    const long blocks = grouped_blocks(p, BI, BJ, grouped_sums(FORM));
+    if (walks ? blocks >= MOST_WALKED_TILES : !grid_fits(blocks, 512)) return hipErrorInvalidConfiguration;
     p.most_tiles = (int)blocks;
     // Workgroups that walk their tiles request the next one's first slots ahead of the stores (16384 rows, 8 groups, 4096 x 4096, bf16:
     // 456 us -> 433).  A ragged sum's sums are shorter than its stores, which the loop's loads then wait for (vmcnt counts in
     // order): 238 us -> 291 for 8198 rows, 16 groups, 2048 x 4096.  With 4 bits the registers do not suffice in the largest tile.
-    hipLaunchKernelGGL((k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>), dim3((unsigned)(grouped_walks(OP::scaled, FORM) ? std::min(blocks, 256l) : blocks)), dim3(512), lds, s, p);
+    hipLaunchKernelGGL((k_grouped_tile<OP, BI, BJ, WI, WJ, NX, NY, FORM, DT>), dim3((unsigned)(walks ? std::min(blocks, 256l) : blocks)), dim3(512), lds, s, p);
     return hipGetLastError();
 }
 

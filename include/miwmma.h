@@ -377,7 +377,9 @@ enum { MIW_EPILOGUE_NONE = 0, MIW_EPILOGUE_GATED_SILU = 1 };
    MIW_ROW_MAJOR (the same weights in the gradient to the rows: dX = dY * W).  rows: sorted positions there are at most (D's
    rows); those outside the groups are not touched.  a_rows: rows of A, those that gather names (0: as many as `rows`).
    offsets outside 0 .. rows and gather outside 0 .. a_rows - 1 are taken as the nearest value inside.  d_type: dtype or MIW_F32; sums are Float32.
-   Any sizes; 16-byte aligned operands with k, n and pitches in multiples of 8 elements run on the faster kernels. */
+   Any sizes; 16-byte aligned operands with k, n and pitches in multiples of 8 elements run on the faster kernels.
+   A launch that would need 2^23 tiles of 256 x 256 results or more (4-bit products, miw_grouped_wgrad; groups do not share tiles), or 2^24 of
+   64 x 64 where sizes or alignment leave only the slowest kernel, is refused with the HIP runtime's error for it. */
 int miw_grouped_gemm(int dtype, int d_type, int w_layout, int epilogue, int64_t rows, int groups, int64_t n, int64_t k,
                      int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldd, int64_t a_rows, const void *A, const void *W,
                      void *D, const int *offsets, const int *gather, void *stream);

@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from grouped_choice import grouped_kernel
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 SCALES = """
@@ -59,3 +61,35 @@ def test_route_workspace_never_falls_as_tokens_grow(miw, experts):
     need = [miw.EXPERTS.route_workspace(t, experts, 1) for t in [*range(0, 20000), *(1 << b for b in range(15, 31))]]
     assert not any(need[:65]) and need[65] > 0
     assert all(a <= b for a, b in zip(need, need[1:]))
+
+
+# Sizes up to what the entries accept, and matrices that a GPU's memory holds.
+GROUPS, WIDTHS, DEPTHS, ROWS = (1, 3, 64, 1024, 8192, 65536), (8, 64, 336, 2016, 2056, 8192, 32768), (8, 32, 64, 2048, 16384), (1, 10, 700, 65536, 600000)
+
+
+@pytest.mark.parametrize("kind", ["16 bits", "4 bits", "sum"])
+def test_the_kernel_that_is_chosen_can_be_launched(miw, kind):
+    seen = set()
+    for groups in GROUPS:
+        for n in WIDTHS:
+            for k in DEPTHS:
+                for rows in ROWS:
+                    if groups * n * (n if kind == "sum" else k) > 1 << 37 or rows * max(n, k) > 1 << 37:
+                        continue
+                    tiles = -(-n // 256) * (min(groups, rows) + rows // 256 if kind != "sum" else groups * -(-n // 256))
+                    if kind != "16 bits" and tiles >= (1 << 23) - 8:  # (refused)
+                        continue
+                    sizes = dict(m=n, n=n) if kind == "sum" else dict(n=n, k=k, layout="col")
+                    name, workgroups, threads = grouped_kernel(miw, rows=rows, groups=groups, mxfp4=kind == "4 bits", **sizes)
+                    seen.add(name)
+                    walks = name.startswith("tile") and kind == "16 bits"
+                    assert workgroups < 1 << 30 if walks else workgroups * threads < 1 << 32, (kind, groups, n, k, rows, name, workgroups)
+    assert len(seen) > 3, seen
+
+
+def test_many_groups_of_few_rows(miw):
+    """As many groups as the products take, nearly all of them without rows."""
+    for mxfp4 in (False, True):
+        for n in (2016, 2056, 4096, 65536):
+            name, workgroups, threads = grouped_kernel(miw, rows=10, groups=65536, n=n, k=64, mxfp4=mxfp4)
+            assert workgroups * threads < 1 << 32, (n, name, workgroups)

@@ -27,3 +27,35 @@ def test_mxfp4_grouped_gemm_panels_of_all_groups(gpu, rows, groups, n, k):
     for g in range(groups):
         r = slice(offsets[g], offsets[g + 1])
         assert np.array_equal(got[r], x[r] @ w[g].T), g
+
+
+@pytest.mark.parametrize("kind", ["f16", "mxfp4"])
+def test_many_groups_without_rows(gpu, kind):
+    """65536 groups, ten rows, wide weights: memory for all of them, and numbers in those that have rows."""
+    groups, n, k, E, Q, rng = 65536, 2056, 32, gpu.EXPERTS, gpu.MXFP4, np.random.default_rng(3)
+    used, lib = np.array([0, 1, 4097, 30000, 65535]), gpu._lib.load()
+    sizes = np.zeros(groups, np.int64)
+    sizes[used] = [1, 3, 1, 3, 2]
+    offsets = upload(gpu, np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32))
+    a, w = rng.integers(-2, 3, (10, k)).astype(np.float16), rng.integers(-2, 3, (len(used), n, k)).astype(np.float16)
+    D = upload(gpu, np.full((10, n), 99, np.float32))
+
+    def spread(parts):
+        parts = np.ascontiguousarray(parts).reshape(len(used), -1).view(np.uint8)
+        out = gpu.DeviceArray.undef(np.uint8, groups * parts.shape[1])
+        for g, part in zip(used, parts):
+            assert lib.miw_memcpy_h2d(out.ptr + int(g) * parts.shape[1], part.ctypes.data, part.nbytes) == 0
+        return out
+
+    if kind == "f16":
+        E.grouped_gemm(upload(gpu, a), spread(w), D, offsets, rows=10, groups=groups, n=n, k=k, d_type=np.float32)
+    else:
+        quantized = [ref.quantize(x.astype(float)) for x in (a, *w)]
+        assert all(np.array_equal(q[2], x) for q, x in zip(quantized, (a, *w)))
+        Q.grouped_gemm(upload(gpu, quantized[0][0]), upload(gpu, ref.panels(quantized[0][1])), spread([q[0] for q in quantized[1:]]), spread([ref.panels(q[1]) for q in quantized[1:]]), D,
+                       offsets, rows=10, groups=groups, n=n, k=k, d_type=np.float32)
+    got, at = D.to_host().reshape(10, n), 0
+    for g, x in zip(used, w):
+        for _ in range(sizes[g]):
+            assert np.array_equal(got[at], x.astype(float) @ a[at].astype(float)), (g, at)
+            at += 1
