@@ -165,7 +165,6 @@ int miw_route_grad(int dtype, int64_t tokens, int experts, int top, int64_t ld, 
     CHECK(check_element("route_grad", "gates", gates, 4));
     CHECK(check_element("route_grad", "dgates", dgates, 4));
     CHECK(check_element("route_grad", "dlogits", dlogits, type_size(dtype)));
-    if (tokens >= 1 << 25) return api_fail(MIW_ERR_UNSUPPORTED, "route_grad: %lld tokens do not fit the launch grid", (long long)tokens);
     REQUIRE_INIT("route_grad");
     const miw::route_grad_params p{logits, chosen, gates, dgates, dlogits, (int)tokens, experts, top, over_all != 0, ld, ldd};
     HIP_TRY(miw::launch_route_grad(p, dtype, (hipStream_t)stream));

@@ -59,3 +59,29 @@ def test_many_groups_without_rows(gpu, kind):
         for _ in range(sizes[g]):
             assert np.array_equal(got[at], x.astype(float) @ a[at].astype(float)), (g, at)
             at += 1
+
+
+def test_route_and_its_gradient_of_2_to_25_tokens(gpu):
+    """More tokens than one pass of the grid: a batch of tokens over and over gives that batch's results over and over."""
+    E, rng = gpu.EXPERTS, np.random.default_rng(8)
+    part, times, experts, top = 1 << 15, 1 << 10, 5, 2
+    z, dg = rng.normal(size=(part, experts)).astype(np.float16), rng.normal(size=(part, top)).astype(np.float32)
+    out = []
+    for n, more in ((1, 0), (times, 7)):
+        tokens = part * n + more
+        repeat = lambda a: upload(gpu, np.concatenate([np.tile(a, (n, 1)), a[:more]]))  # noqa: E731
+        new = lambda T, *shape: gpu.DeviceArray.undef(T, int(np.prod(shape)))  # noqa: E731
+        sizes = dict(tokens=tokens, experts=experts, top=top, dtype=np.float16, over_all=True)
+        Z, chosen, gates, offsets, rows, place = repeat(z), new(np.int32, tokens, top), new(np.float32, tokens, top), new(np.int32, experts + 1), new(np.int32, tokens, top), new(np.int32, tokens, top)
+        dz = new(np.float16, tokens, experts)
+        E.route(Z, chosen, gates, offsets, rows, place, workspace=new(np.uint8, E.route_workspace(tokens, experts, top)), **sizes)
+        E.route_grad(Z, chosen, gates, repeat(dg), dz, **sizes)
+        out.append([v.to_host() for v in (chosen, gates, dz)] + [offsets.to_host(), place.to_host()])
+    small, large = out
+    for s, l in zip(small[:3], large[:3]):
+        assert np.array_equal(l[:len(s) * times].reshape(times, -1), np.broadcast_to(s, (times, len(s)))) and np.array_equal(l[len(s) * times:], s[:len(l) - len(s) * times])
+    # the sorted position of each choice: those of its expert from the first on, in the order of tokens
+    chosen, offsets, place = large[0], large[3], large[4]
+    for e in range(experts):
+        assert np.array_equal(place[chosen == e], np.arange(offsets[e], offsets[e + 1]))
+    assert offsets[0] == 0 and offsets[-1] == len(chosen)
