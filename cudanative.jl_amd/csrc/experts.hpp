@@ -98,8 +98,8 @@ hipError_t launch_grouped_tile_bf16(const grouped_params &p, grouped_tile_size t
 hipError_t launch_grouped_tile_mxfp4(const grouped_params &p, grouped_tile_size t, int d_type, hipStream_t s);
 hipError_t launch_grouped_plain(grouped_params p, int dtype, int d_type, bool ragged_sum, hipStream_t s);
 hipError_t launch_grouped_mxfp4_plain(grouped_params p, int d_type, hipStream_t s);
-// Groups of few rows.  mt: 16-row tiles taken together (1, 2, 4); wt: 16-row tiles of weights a workgroup, with wt 2 on 2 or 4
-// wavefronts, with wt 1 on 8.
+// Groups of few rows.  mt: 16-row tiles taken together; wt: 16-row tiles of weights a workgroup.  There are mt 1 with wt 2 on 2 or 4 wavefronts,
+// and mt 1, 2 and 4 with wt 1 on 8.
 struct grouped_narrow_form {
     int mt, wt, waves;
 };

@@ -154,15 +154,12 @@ template <class OP, class DT>
 static hipError_t launch_narrow_type(const grouped_params &p, grouped_narrow_form f, hipStream_t s)
 {
     const long blocks = (long)p.groups * ((p.I + 16 * f.wt - 1) / (16 * f.wt));
-    auto with_rows = [&](auto mt) {
-        constexpr int MT = decltype(mt)::value;
-        if (f.wt == 1) hipLaunchKernelGGL((k_grouped_narrow<OP, MT, 1, 8, 2, DT>), dim3((unsigned)blocks), dim3(512), 0, s, p);
-        else if (f.waves == 4) hipLaunchKernelGGL((k_grouped_narrow<OP, MT, 2, 4, 2, DT>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((k_grouped_narrow<OP, MT, 2, 2, 2, DT>), dim3((unsigned)blocks), dim3(128), 0, s, p);
-    };
-    if (f.mt == 1) with_rows(std::integral_constant<int, 1>{});
-    else if (f.mt == 2) with_rows(std::integral_constant<int, 2>{});
-    else with_rows(std::integral_constant<int, 4>{});
+    const dim3 grid((unsigned)blocks), block((unsigned)(64 * f.waves));
+    if (f.wt == 2 && f.waves == 2) hipLaunchKernelGGL((k_grouped_narrow<OP, 1, 2, 2, 2, DT>), grid, block, 0, s, p);
+    else if (f.wt == 2) hipLaunchKernelGGL((k_grouped_narrow<OP, 1, 2, 4, 2, DT>), grid, block, 0, s, p);
+    else if (f.mt == 1) hipLaunchKernelGGL((k_grouped_narrow<OP, 1, 1, 8, 2, DT>), grid, block, 0, s, p);
+    else if (f.mt == 2) hipLaunchKernelGGL((k_grouped_narrow<OP, 2, 1, 8, 2, DT>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((k_grouped_narrow<OP, 4, 1, 8, 2, DT>), grid, block, 0, s, p);
     return hipGetLastError();
 }
 

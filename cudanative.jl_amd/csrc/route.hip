@@ -404,13 +404,12 @@ static int route_chunks(long tokens)
     return tokens <= ROUTE_TOKENS ? 1 : (int)((tokens + route_chunk(tokens) - 1) / route_chunk(tokens));
 }
 
+// Registers that hold a token's logits on sixteen lanes (up to 256 experts); a wavefront has sixteen for up to 1024.
 template <class F>
 static void with_registers(int experts, F go)
 {
-    const int r = (experts + 63) / 64;
-    if (r == 1) go(std::integral_constant<int, 1>{});
-    else if (r == 2) go(std::integral_constant<int, 2>{});
-    else if (r <= 4) go(std::integral_constant<int, 4>{});
+    if (experts <= 64) go(std::integral_constant<int, 4>{});
+    else if (experts <= 128) go(std::integral_constant<int, 8>{});
     else go(std::integral_constant<int, 16>{});
 }
 template <class F>
@@ -434,7 +433,7 @@ hipError_t launch_route(route_params p, int dtype, hipStream_t s)
             else hipLaunchKernelGGL((k_route_choose<T, R, ROW, false>), dim3((unsigned)p.chunks), dim3(ROUTE_THREADS), 0, s, p);
         };
         if (p.experts > 256) go(std::integral_constant<int, 16>{}, std::false_type{});
-        else with_registers(p.experts, [&](auto regs) { go(std::integral_constant<int, 4 * decltype(regs)::value>{}, std::true_type{}); });
+        else with_registers(p.experts, [&](auto regs) { go(regs, std::true_type{}); });
     });
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.chunks == 1) return e;
@@ -450,7 +449,7 @@ hipError_t launch_route_grad(const route_grad_params &p, int dtype, hipStream_t 
     with_type(dtype, [&](auto type) {
         using T = decltype(type);
         if (row) with_registers(p.experts, [&](auto regs) {
-            hipLaunchKernelGGL((k_route_grad<T, 4 * (decltype(regs)::value < 4 ? decltype(regs)::value : 4), 16>), grid, block, 0, s, p);
+            hipLaunchKernelGGL((k_route_grad<T, decltype(regs)::value, 16>), grid, block, 0, s, p);
         });
         else hipLaunchKernelGGL((k_route_grad<T, 16, 64>), grid, block, 0, s, p);
     });

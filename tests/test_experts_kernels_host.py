@@ -1,5 +1,6 @@
 """Functions of the grouped products' kernels and dispatch that also run on the host: addresses and choices of kernels, without a GPU."""
 import os
+import re
 import shutil
 import subprocess
 
@@ -93,3 +94,37 @@ def test_many_groups_of_few_rows(miw):
         for n in (2016, 2056, 4096, 65536):
             name, workgroups, threads = grouped_kernel(miw, rows=10, groups=65536, n=n, k=64, mxfp4=mxfp4)
             assert workgroups * threads < 1 << 32, (n, name, workgroups)
+
+
+def _instances(miw, kernel):
+    """Template arguments of a kernel's instances in the library (those with a 16-bit type of results have names that nm may not take apart)."""
+    nm = shutil.which("nm")
+    if nm is None:
+        pytest.skip("no nm")
+    names = subprocess.run([nm, "-C", miw._lib.LIB_PATH], capture_output=True, text=True, check=True).stdout
+    return {tuple(x.strip() for x in args.split(",")) for args in re.findall(r"__device_stub__%s<(.*)>\(" % kernel, names)}
+
+
+def _chosen(miw, **form):
+    return {grouped_kernel(miw, rows=rows, groups=groups, n=n, k=k, **form)[0]
+            for groups in (1, 3, 8, 16, 64, 128) for n in (64, 256, 336, 1024, 2048, 4096) for k in (32, 512, 2048, 8192) for rows in (1, 24, 64, 100, 500, 1000, 3000, 16384, 65536)}
+
+
+@pytest.mark.parametrize("op,mxfp4", [("op_f16", False), ("op_bf16", False), ("op_mxfp4", True)])
+def test_every_grouped_kernel_of_the_library_is_chosen_for_some_product(miw, op, mxfp4):
+    chosen = _chosen(miw, mxfp4=mxfp4)
+    forms = {"narrow %s %s %s" % a[1:4] for a in _instances(miw, "k_grouped_narrow") if a[0].endswith(op)}
+    assert forms == {c for c in chosen if c.startswith("narrow")}
+    tiles = {a[1:3] + (a[7],) for a in _instances(miw, "k_grouped_tile") if a[0].endswith(op)}  # (extents and form)
+    reached = {("col", c) for c in chosen}
+    if not mxfp4:
+        reached |= {("row", c) for c in _chosen(miw, layout="row")}
+        reached |= {("sum", c) for c in {grouped_kernel(miw, rows=rows, groups=groups, n=n, m=m)[0] for groups in (1, 8, 64) for n in (64, 336, 1024, 4096) for m in (64, 1024, 4096)
+                                         for rows in (1, 100, 1000, 16384)}}
+    assert tiles == {tuple(c.split()[1].split("x")) + ({"col": "0", "row": "1", "sum": "3" if c == "tile 256x128" else "2"}[form],) for form, c in reached if c.startswith("tile")}
+
+
+def test_every_routing_kernel_of_the_library_is_launched_for_some_experts(miw):
+    """Sixteen lanes a token hold 16 experts a register up to 256 experts, a wavefront 64 beyond."""
+    forms = {a[1:3] for a in _instances(miw, "k_route_choose")}
+    assert forms == {("4", "true"), ("8", "true"), ("16", "true"), ("16", "false")}
