@@ -27,10 +27,11 @@ constexpr int ROUTE_SEGMENTS = ROUTE_TOKENS * ROUTE_TOP / 64;         // of 64 c
 static_assert(ROUTE_SEGMENTS <= ROUTE_WAVES, "a wavefront for each");
 constexpr float LARGEST = 3.4028234663852886e38f;
 
-// Key of a logit: the order of the keys is that of the values, -0 equals 0, and what is never chosen has key 0.
+// Key of a logit: the order of the keys is that of the values, -0 equals 0, +inf the largest finite Float32, and what is never
+// chosen has key 0.
 __device__ inline unsigned order_key(float z)
 {
-    const unsigned u = __builtin_bit_cast(unsigned, z + 0.0f);  // (-0 becomes 0)
+    const unsigned u = __builtin_bit_cast(unsigned, fminf(z, LARGEST) + 0.0f);  // (-0 becomes 0)
     const unsigned key = u & 0x80000000u ? ~u : u | 0x80000000u;
     return z > -__builtin_inff() ? key : 0u;  // (false for NaN)
 }
@@ -40,7 +41,7 @@ __device__ inline float key_value(unsigned key)
 }
 
 // Logits of 16 bits have keys of 16, and the expert fits beside them: the largest such number names the largest logit and, of equal ones,
-// the lowest expert, by one reduction.
+// the lowest expert, by one reduction.  (No finite one equals Float32's largest, which +inf counts as.)
 template <class T>
 __device__ inline unsigned packed_key(T z, int expert)
 {
@@ -92,7 +93,7 @@ __device__ inline void choose_row(const route_params &p, int base, int first, in
     constexpr bool PACKED = sizeof(T) == 2;
     auto value_of = [](unsigned k) {
         if constexpr (PACKED) return fminf(packed_value<T>(k), LARGEST);
-        else return fminf(key_value(k), LARGEST);
+        else return key_value(k);
     };
     unsigned key[R];
 #pragma unroll
@@ -162,12 +163,12 @@ __device__ inline void choose_wave(const route_params &p, int base, int token, i
             const unsigned long has = __ballot(key[i] == most);
             if (has) expert = 64 * i + __builtin_ctzl(has);
         }
-        const float v = fminf(key_value(most), LARGEST);
+        const float v = key_value(most);
         if (j == 0) {
             largest = v;
             if (p.over_all)
 #pragma unroll
-                for (int i = 0; i < R; i++) every += key[i] ? __expf(fminf(key_value(key[i]), LARGEST) - v) : 0.f;
+                for (int i = 0; i < R; i++) every += key[i] ? __expf(key_value(key[i]) - v) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < R; i++)
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(256) void k_route_grad(route_grad_params p)
 #pragma unroll
             for (int i = 0; i < R; i++) most = max(most, order_key(v[i]));
             most = LANES == 16 ? row_max(most) : wave_max(most);
-            const float largest = most ? fminf(key_value(most), LARGEST) : 0.f;
+            const float largest = most ? key_value(most) : 0.f;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < R; i++) {

@@ -85,3 +85,20 @@ def test_route_and_its_gradient_of_2_to_25_tokens(gpu):
     for e in range(experts):
         assert np.array_equal(place[chosen == e], np.arange(offsets[e], offsets[e + 1]))
     assert offsets[0] == 0 and offsets[-1] == len(chosen)
+
+
+@pytest.mark.parametrize("experts", [8, 300])
+def test_route_takes_infinity_for_the_largest_float(gpu, experts):
+    """+inf counts as the largest finite Float32: the two are equal, and the lower expert goes first."""
+    E, top = gpu.EXPERTS, 4
+    most = np.finfo(np.float32).max
+    z = np.zeros((3, experts), np.float32)
+    z[0, [1, 3, 5]] = most, np.inf, most
+    z[1, [0, experts - 1]] = np.inf, most
+    z[2, [2, experts - 2]] = most, np.inf
+    want = ref.route(z.astype(np.float64), top, False)
+    for over_all in (False, True):
+        out = [upload(gpu, np.zeros(n, t)) for n, t in ((3 * top, np.int32), (3 * top, np.float32), (experts + 1, np.int32), (3 * top, np.int32), (3 * top, np.int32))]
+        E.route(upload(gpu, z), *out, tokens=3, experts=experts, top=top, over_all=over_all)
+        assert np.array_equal(out[0].to_host().reshape(3, top), want[0])
+        assert np.allclose(out[1].to_host().reshape(3, top), want[1], rtol=1e-6, atol=0)
