@@ -56,6 +56,17 @@ __device__ inline float packed_value(unsigned packed)
     return (float)__builtin_bit_cast(T, (unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
 }
 
+// exp of x <= 0, -inf among them, to two units in the last place: 2^t with t = x log2 e rounded, times what the rounding left out, which for x
+// near -80 is up to 2^-18 of the result.  Results below 2^-126 are zeros.  (Gradient of 16381 tokens of 1024 experts over all, bf16: 33.7 us with 2^t alone,
+// 34.7 so, 36.9 with expf.)
+__device__ inline float exp_below(float x)
+{
+    constexpr float LOG2E = 1.44269504f, REST = (float)(1.4426950408889634074 - (double)LOG2E), LN2 = 0.69314718f;
+    x = fmaxf(x, -200.f);
+    const float t = x * LOG2E, left = __builtin_fmaf(x, REST, __builtin_fmaf(x, LOG2E, -t)), e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, LN2 * left, e);
+}
+
 // Over the sixteen lanes of a row, to all of them; sums pair the same lanes in every lane.
 template <class F>
 __device__ inline int row_reduce(int v, F join)
@@ -114,7 +125,7 @@ __device__ inline void choose_row(const route_params &p, int base, int first, in
             largest = v;
             if (p.over_all)
 #pragma unroll
-                for (int i = 0; i < R; i++) every += key[i] ? __expf(value_of(key[i]) - v) : 0.f;
+                for (int i = 0; i < R; i++) every += exp_below(key[i] ? value_of(key[i]) - v : -__builtin_inff());
         }
         int expert;
         if constexpr (PACKED) {
@@ -135,7 +146,7 @@ __device__ inline void choose_row(const route_params &p, int base, int first, in
             value = v;
         }
     }
-    const float part = mine >= 0 ? __expf(value - largest) : 0.f;
+    const float part = mine >= 0 ? exp_below(value - largest) : 0.f;
     const float sum = row_sum(p.over_all ? every : part);
     if (in) write_choice(p, base, token, lane, mine, part, sum, kept);
 }
@@ -168,7 +179,7 @@ __device__ inline void choose_wave(const route_params &p, int base, int token, i
             largest = v;
             if (p.over_all)
 #pragma unroll
-                for (int i = 0; i < R; i++) every += key[i] ? __expf(key_value(key[i]) - v) : 0.f;
+                for (int i = 0; i < R; i++) every += exp_below(key[i] ? key_value(key[i]) - v : -__builtin_inff());
         }
 #pragma unroll
         for (int i = 0; i < R; i++)
@@ -178,7 +189,7 @@ __device__ inline void choose_wave(const route_params &p, int base, int token, i
             value = v;
         }
     }
-    const float part = mine >= 0 ? __expf(value - largest) : 0.f;
+    const float part = mine >= 0 ? exp_below(value - largest) : 0.f;
     write_choice(p, base, token, lane, mine, part, wave_sum(p.over_all ? every : part), kept);
 }
 
@@ -365,7 +376,7 @@ __global__ __launch_bounds__(256) void k_route_grad(route_grad_params p)
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                v[i] = v[i] > -__builtin_inff() ? __expf(fminf(v[i], LARGEST) - largest) : 0.f;  // (NaN: 0)
+                v[i] = exp_below(v[i] > -__builtin_inff() ? fminf(v[i], LARGEST) - largest : -__builtin_inff());  // (NaN: 0)
                 sum += v[i];
             }
             const float total = LANES == 16 ? row_sum(sum) : wave_sum(sum);

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import experts_oracle as ref
-from experts_oracle import upload
+from experts_oracle import KINDS, upload
 from test_gpu_experts import _sizes_of
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +102,37 @@ def test_route_takes_infinity_for_the_largest_float(gpu, experts):
         E.route(upload(gpu, z), *out, tokens=3, experts=experts, top=top, over_all=over_all)
         assert np.array_equal(out[0].to_host().reshape(3, top), want[0])
         assert np.allclose(out[1].to_host().reshape(3, top), want[1], rtol=1e-6, atol=0)
+
+
+# Units of 2^-24 of a gate: exp is off by at most one unit in the last place (2) of the numerator and of each summand (2), the sum takes at
+# most sixteen registers' and four lanes' additions (20), the quotient is rounded once (1).  The differences of these logits are exact.
+GATE = 25 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("experts", [8, 120, 700])
+@pytest.mark.parametrize("over_all", [False, True])
+def test_small_gates_keep_their_bits(gpu, experts, kind, over_all):
+    """Logits as far as 84 below the largest: gates of 10^-36 are as precise as gates of one half."""
+    kind, rng = KINDS[kind], np.random.default_rng(experts)
+    tokens, top, E = 40, 8, gpu.EXPERTS
+    # multiples of 1/2 that every type holds; eight of them above the others
+    z = np.full((tokens, experts), -45.0)
+    z[:, :8] = rng.integers(-88, 81, (tokens, 8)) / 2
+    z[:, 0] = 40.0
+    out = [upload(gpu, np.zeros(n, t)) for n, t in ((tokens * top, np.int32), (tokens * top, np.float32), (experts + 1, np.int32), (tokens * top, np.int32), (tokens * top, np.int32))]
+    Z, dgates, dz = upload(gpu, kind.store(z)), np.zeros((tokens, top), np.float32), upload(gpu, np.zeros((tokens, experts), kind.dtype))
+    E.route(Z, *out, tokens=tokens, experts=experts, top=top, dtype=kind.marker(gpu), over_all=over_all)
+    chosen, gates = (v.to_host().reshape(tokens, top) for v in out[:2])
+    want = ref.route(z, top, over_all)
+    assert np.array_equal(chosen, want[0])
+    far = np.abs(gates - want[1]) / want[1]
+    assert far.max() <= GATE, far.max() * 2.0 ** 24
+    # the gradient from the largest choice alone: minus the product of two gates for every other one, in Float32 two gates' errors, a sum of sixteen
+    # products and three roundings
+    dgates[:, 0] = 1.0
+    E.route_grad(Z, out[0], out[1], upload(gpu, dgates), dz, tokens=tokens, experts=experts, top=top, dtype=kind.marker(gpu), over_all=over_all)
+    exact = ref.route_grad(z, want[0], dgates.astype(np.float64), over_all)
+    others = (z < 40) & (exact != 0)
+    far = np.abs(kind.load(dz.to_host().reshape(tokens, experts)) - exact)[others] - kind.roundoff * 1.01 * np.abs(exact[others])
+    assert np.all(far <= (2 * GATE + 8 * 2.0 ** -24) * np.abs(exact[others]) + (2.0 ** -25 if kind.name == "f16" else 0.0))
