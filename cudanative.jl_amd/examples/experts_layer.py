@@ -60,14 +60,17 @@ class ExpertsLayer:
     # ---- weights and activations in 4 bits
 
     def pack(self, stream=None):
-        """Both weights in 4 bits, once.  All experts' matrices are one tall matrix to the quantisation, and lie one behind the
-        other in each panel of its scales."""
+        """Both weights in 4 bits, once.  All experts' matrices lie one behind the other in each panel of scales, every one on an even row;
+        where their rows are even in number they are one tall matrix to the quantisation."""
         Q, new = self.pkg.MXFP4, self.pkg.DeviceArray.undef
         self.packed = []
         for W, n, k in ((self.W1, 2 * self.hidden, self.width), (self.W2, self.width, self.hidden)):
-            codes, scales = new(np.uint8, Q.codes_bytes(self.experts * n, k)), new(np.uint8, Q.scales_bytes(self.experts * n, k))
-            Q.quantize(W, codes, scales, rows=self.experts * n, k=k, stream=stream)
-            self.packed.append((codes, scales, dict(n=n, k=k, lds_w=self.experts * n + self.experts * n % 2, stride_ws=8 * n)))
+            own = n + n % 2
+            lds, at_once, first = self.experts * own, self.experts if own == n else 1, getattr(W, "ptr", W)
+            codes, scales = new(np.uint8, Q.codes_bytes(self.experts * n, k)), new(np.uint8, Q.scales_bytes(lds, k))
+            for e in range(0, self.experts, at_once):
+                Q.quantize(first + 2 * e * n * k, codes.ptr + Q.codes_bytes(e * n, k), scales.ptr + 8 * e * own, rows=at_once * n, k=k, lds=lds, stream=stream)
+            self.packed.append((codes, scales, dict(n=n, k=k, lds_w=lds, stride_ws=8 * own)))
         self.x4 = new(np.uint8, Q.codes_bytes(self.tokens, self.width)), new(np.uint8, Q.scales_bytes(self.tokens, self.width))
         rows = self.tokens * self.top
         self.a4 = new(np.uint8, Q.codes_bytes(rows, self.hidden)), new(np.uint8, Q.scales_bytes(rows, self.hidden))

@@ -2,9 +2,9 @@
 import numpy as np
 import pytest
 
-import experts_oracle as ref
+import test_gpu_experts_layer as layer_tests
 from experts_oracle import upload
-from test_gpu_experts_layer import LAYER, Layer64, _far, _inputs, example  # noqa: F401 (a fixture)
+from test_gpu_experts_layer import example  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,10 @@ def test_calls_of_fewer_tokens_than_the_layer_was_made_for(gpu, example):  # noq
         for got, want in zip(layer.backward(x, logits, dy, tokens=tokens), own.backward(x, logits, dy, tokens=tokens)):
             want = want.to_host()
             assert np.array_equal(got.to_host()[:len(want)], want), tokens
+
+
+# Widths of an odd number of columns, whose matrices of 4-bit weights start on even rows of their panels; few and many rows an expert.
+@pytest.mark.parametrize("tokens,experts,top,width,hidden", [(9, 4, 2, 35, 11), (70, 3, 2, 301, 145), (400, 5, 2, 129, 67)])
+def test_odd_widths(gpu, example, tokens, experts, top, width, hidden):  # noqa: F811
+    layer_tests.test_serving_in_4_bits(gpu, example, tokens, experts, top, width, hidden, True)
+    layer_tests.test_training_step(gpu, example, tokens, experts, top, width, hidden, True)
