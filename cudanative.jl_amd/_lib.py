@@ -201,6 +201,15 @@ def load():
     return _lib
 
 
+def stream_handle(stream):
+    """A Stream object or a raw hipStream_t (None: the default stream) as the C ABI takes it.  An array or a typed pointer is none, though ctypes
+    would take its address."""
+    handle = getattr(stream, "handle", stream)
+    if hasattr(handle, "_as_parameter_"):
+        raise ctypes.ArgumentError("a stream is a Stream or a raw handle, got a %s" % type(stream).__name__)
+    return handle
+
+
 def last_error():
     return load().miw_last_error().decode("utf-8", "replace")
 

@@ -13,6 +13,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
+from ._lib import stream_handle as _stream_handle
 from .array import DeviceArray, DevicePtr
 
 WAVEFRONT = 64
@@ -43,10 +44,6 @@ class Stream:
                 _lib.load().miw_stream_destroy(h)
             except Exception:
                 pass
-
-
-def _stream_handle(stream):
-    return stream.handle if isinstance(stream, Stream) else stream
 
 
 def synchronize(stream=None):

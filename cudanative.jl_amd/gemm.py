@@ -9,6 +9,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
+from ._lib import stream_handle as _stream
 from .array import DeviceArray
 from .wmma import ColMajor, RowMajor, get_hl_frag_info, get_hl_layout, Float16, Float32
 
@@ -20,11 +21,6 @@ def _layout_code(L):
 
 def _dtype_code(T):
     return _lib.F16 if np.dtype(T) == np.float16 else _lib.F32
-
-
-def _stream(stream):
-    """A Stream object or a raw hipStream_t (None: the default stream) as the C ABI takes it."""
-    return getattr(stream, "handle", stream)
 
 
 def _ptr(x):
