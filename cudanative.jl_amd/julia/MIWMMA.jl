@@ -826,6 +826,8 @@ end
 
 const ELEMENT_CODES = Dict(:f16 => Cint(0), :f32 => Cint(1), :bf16 => Cint(2))
 address(x) = x === nothing ? C_NULL : x.ptr
+buffer_bytes(::Nothing) = 0
+buffer_bytes(a::DeviceBuffer{T}) where {T} = length(a) * sizeof(T)
 epilogue_code(e::Symbol) = e === :none ? Cint(0) : e === :gated_silu ? Cint(1) : throw(ArgumentError("epilogue is :none or :gated_silu"))
 
 "Bytes of workspace that route! needs (0: none)."
@@ -837,7 +839,7 @@ end
 
 "The `top` largest logits of each token, their softmax, and the order of the rows by expert."
 function route!(chosen, gates, offsets, rows, place, logits; tokens::Integer, experts::Integer, top::Integer, dtype::Symbol=:f32,
-                ld::Integer=0, over_all::Bool=false, workspace=nothing, workspace_bytes::Integer=0, stream=C_NULL)
+                ld::Integer=0, over_all::Bool=false, workspace=nothing, workspace_bytes::Integer=buffer_bytes(workspace), stream=C_NULL)
     GC.@preserve chosen gates offsets rows place logits workspace check(ccall((:miw_route, libmiwmma), Cint,
         (Cint, Int64, Cint, Cint, Int64, Cint, Ptr{Cvoid}, Ptr{Cint}, Ptr{Cfloat}, Ptr{Cint}, Ptr{Cint}, Ptr{Cint}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}),
         ELEMENT_CODES[dtype], tokens, experts, top, ld, over_all ? 1 : 0, address(logits), address(chosen), address(gates), address(offsets),
