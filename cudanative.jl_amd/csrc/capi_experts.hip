@@ -26,7 +26,7 @@ bool any_type(int t) { return half_type(t) || t == MIW_F32; }
 long type_size(int t) { return t == MIW_F32 ? 4 : 2; }
 bool aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-constexpr int64_t EXTENT = 1 << 26;      // of a matrix' rows
+constexpr int64_t EXTENT = 1 << 26;      // columns of a matrix, and lengths of sums
 constexpr int64_t POSITIONS = 1 << 30;   // rows of a matrix
 constexpr int64_t PITCH = 1ll << 30;     // elements or bytes from row to row
 constexpr int64_t STRIDE = 1ll << 40;    // from group to group

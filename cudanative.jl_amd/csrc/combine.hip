@@ -1,8 +1,8 @@
 // The experts' answers joined by their weights, and the gradients to answers and weights.
 //
 // Bound by HBM: every row of H is read once and every row of the result written once, in 16-byte pieces.  8191 tokens, 4
-// choices, 4096 columns (bf16): 56 us (336 MB, 6.0 TB/s), gradients 105 us (604 MB, 5.7 TB/s); a large copy reaches 5.0 to 5.4.
-// 16 tokens: 2.9 us, a launch's latency and two dependent reads.  Sums run over a
+// choices, 4096 columns (bf16): 56 to 57 us (336 MB, 5.9 TB/s), gradients 105 to 107 us (604 MB, 5.7 TB/s); a large copy reaches 4.8 to 5.4.
+// 16 tokens: 2.9 to 3.2 us, a launch's latency and two dependent reads.  Sums run over a
 // token's choices in order, in Float32, and are rounded once.
 #include "experts.hpp"
 #include "vec_types.hpp"

@@ -6,8 +6,8 @@
 // straight into an MFMA fragment, DEPTH chunks ahead, and the partial sums are added in wavefront order through LDS: no second
 // kernel, the same bits every time.  Which group and which weights a workgroup has is its number: a group without rows costs a
 // look at two offsets.  Registers hold DEPTH * 2 * (WT + MT) * 16 bytes a lane; 16 wavefronts a CU keep some 200 KB on the way.
-// Bound by HBM: 64 rows over 64 groups, 1024 x 2048 (f16): 29 to 34 us for 165 MB, 5.0 to 5.7 TB/s; 4 bits, 128 rows over 64 groups, 2048 x 2048:
-// 22 us for 125 MB.  Partial sums are Float32, rounded once when they are stored.
+// Bound by HBM: 64 rows over 64 groups, 1024 x 2048 (f16): 30 to 35 us for 165 MB, 4.7 to 5.6 TB/s; 4 bits, 128 rows over 64 groups, 2048 x 2048:
+// 22 to 24 us for 125 MB.  One group of 4096 x 4096: 8 rows 9.8 us in f16, 4.7 in 4 bits (weights partly in the last-level cache).  Partial sums are Float32, rounded once when they are stored.
 #pragma once
 #include "grouped_tile.hpp"
 #include <type_traits>

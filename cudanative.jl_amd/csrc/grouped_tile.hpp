@@ -12,12 +12,14 @@
 //     entries travel to LDS NY - 1 slots ahead of the slot that they are for.  A slot is 64 along k, or 32, where half the LDS then
 //     suffices for a tile of 256 x 128 and a CU holds two workgroups: while one waits for its first slot the other multiplies.  Stores
 //     and products add up all the same: 8198 rows, 16 groups, 2048 x 4096 (bf16, Float32 results): without stores 136 to 147 us, stores
-//     alone 111 to 118, both 238 to 258 on 256 x 256 with slots of 64; 224 to 236 on 256 x 128 with slots of 32.
+//     alone 111 to 118, both 238 to 258 on 256 x 256 with slots of 64; 221 to 243 on 256 x 128 with slots of 32.  Added to D: 301, for the 537 MB
+//     more that are read.
 //
-// Sums are Float32 in the accumulators and are rounded once, when they are stored (gated ones after the activation).  Measured: 16384 rows, 8
-// groups, 4096 x 4096 (bf16): 427 to 438 us, 1.26 to 1.29 PFLOP/s, matrix cores busy 67 % of the cycles, which is what the power cap leaves a dense product
-// too.  The gradient to 8198 rows, 16 groups, 2048 x 4096 (i contiguous): 157 to 161 us, 0.87 PFLOP/s for 40 tiles of rows where 32 would do.  4 bits,
-// 4096 x 4096 x 8192: 64 to 66 us, 4.2 PFLOP/s; cores 42 %, the memory cluster is the longer one (without loads 55 us, without MFMAs 43).
+// Sums are Float32 in the accumulators and are rounded once, when they are stored (gated ones after the activation).  Measured, back to back on several cards: 16384 rows, 8
+// groups of uneven size, 4096 x 4096 (bf16): 427 to 460 us, 1.20 to 1.29 PFLOP/s, matrix cores busy 65 to 67 % of the cycles at some 1.75 GHz, which is what the power
+// cap leaves a dense product too (even groups: 400 us; gated 410).  The gradient to 8198 rows, 16 groups, 2048 x 4096 (i contiguous): 157 to 172 us, 0.80 to 0.87 PFLOP/s for 40 tiles
+// of rows where 32 would do.  4 bits, 4096 x 4096 x 8192: 64 to 69 us, 4.0 to 4.3 PFLOP/s, gated 73; cores 41 to 43 %, the memory cluster is the longer one (without loads 55 us, without
+// MFMAs 43).  4 bits, 16384 rows, 8 even groups, 4096 x 4096: 156 us, 3.5 PFLOP/s, gated 174; 2048 rows, 16 groups, 2048 x 2048: 15.6, gated 17.9 (f16 42 and 45).
 //
 // Where the sum ends inside a slot, lanes fetch the last valid chunk (row) again and its values are zeroed in both operands'
 // fragments, in a copy of the loop body that only the last slot runs.

@@ -3,8 +3,8 @@
 // A lane has eight values of a block, four lanes the block, 32 lanes a row's piece of one panel of scales (256 values); the
 // largest magnitude meets in the four lanes by data-parallel moves.  The scale is a power of two, so dividing by it is
 // exact, and v_cvt_scalef32_pk_fp4_f32 rounds to the nearest code, ties to the even one, and saturates.
-// Bound by HBM: a Float16 matrix is read once (2 bytes a value) and 17/32 of a byte written.  8192 x 8192 (Float16): 33 us
-// (170 MB, 5.2 TB/s), back to bfloat16 25 us (170 MB, 6.8 TB/s: the codes are still in a cache).
+// Bound by HBM: a Float16 matrix is read once (2 bytes a value) and 17/32 of a byte written.  8192 x 8192 (Float16): 33 to 35 us
+// (170 MB, 4.8 to 5.2 TB/s), back to bfloat16 25 us (170 MB, 6.8 TB/s: the codes are still in a cache).
 #include "experts.hpp"
 #include "vec_types.hpp"
 

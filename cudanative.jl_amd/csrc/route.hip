@@ -10,9 +10,10 @@
 // bit of the expert's number, and what the 64s before it have is added from a table in LDS.  The second adds up the counts of
 // lower experts and earlier chunks and writes the positions.  Counts are integers: no order of theirs matters.
 //
-// Bound by latency throughout: 16381 tokens, 128 experts, 8 choices (bf16): 4.2 MB of logits, 1.6 MB of results:
-// choose 8.5 us (9.4 with two reductions), place 8.0 us, gradient 6.0 us (8.4 MB in and out; with a wavefront a token 7.8) where the bytes alone take one to two each.  16 tokens of 64
-// experts, 4 choices: one launch of 3.2 us.
+// Bound by latency throughout: 16381 tokens, 128 experts, 8 choices (bf16), 4.2 MB of logits and 1.6 MB of results, where the bytes alone take one to two
+// microseconds a launch: back to back choice and order 16.5 us and gradient 6.2 (8.4 MB in and out); under the profiler, medians, choose 9.0, place 8.5 to 9.8,
+// gradient 6.4 to 7.3.  (When they were tried: choose 8.5, 9.4 with two reductions; gradient 6.0, 7.8 with a wavefront a token.)  16 tokens of 64 experts, 4
+// choices: one launch of 3.2 to 3.4 us.  A wavefront a token: 16381 tokens of 512 experts (f32) 70 us, gradient over all 24; of 1024 (bf16) 102 and 35.
 #include "experts.hpp"
 #include "vec_types.hpp"
 

@@ -66,8 +66,9 @@ __device__ inline void store8(T *p, f32x8 v, int count)
     }
 }
 
-// The gate of a gated SiLU times its value.  (__expf is within a few units of Float32's last place over the range in which the
-// result is not a zero, far below the rounding that follows.)
+// The gate of a gated SiLU times its value.  __expf scales its argument in one rounding: the result is off by |gate| 2^-24 of itself and a few units
+// more, twenty of Float32's last place at a gate of -40, as much as half a unit of the gate, a rounded sum, makes; the rounding to 16 bits that mostly follows
+// is far above that.  Gates below -88.7 give zeros.
 __device__ inline float gated_silu(float gate, float value) { return gate / (1.f + __expf(-gate)) * value; }
 
 // Reductions over a wavefront by data-parallel primitives: no LDS, some fifty cycles.  The result is uniform.
