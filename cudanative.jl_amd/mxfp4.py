@@ -2,7 +2,7 @@
 
 A rows x k matrix is two byte arrays.  codes: two values to a byte, the one of the lower k in the low half, rows of 16 *
 ceil(k / 32) bytes.  scales: panels of eight blocks (256 values of k), ceil(k / 256) x (rows rounded up to an even number) x 8
-bytes.  `codes_bytes` and `scales_bytes` say how much memory they take.
+bytes.  `codes_bytes` and `scales_bytes` say how much memory they take.  A last block's values beyond k are zeros: `quantize` writes them, products count on them.
 
 No counterpart in the reference.  Arrays are DeviceArrays or raw device addresses; a pitch or stride of 0 means dense.  All
 calls are asynchronous on `stream`.

@@ -407,7 +407,8 @@ int miw_combine_grad(int dtype, int64_t tokens, int top, int64_t n, int64_t rows
 /* ------------------------------------------------- microscaled 4-bit floats -- */
 /* A matrix of rows x k values of e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with one e8m0 scale for 32 along k.
      codes   two values to a byte, the one of the lower k in the low half; rows of ldq bytes, a multiple of 16 and at least
-             16 * ceil(k / 32), on 16-byte addresses.  What a last block has beyond k is written as zeros.
+             16 * ceil(k / 32), on 16-byte addresses.  What a last block has beyond k is written as zeros, and products take it for zeros
+             without a look: codes from elsewhere have to have them.
      scales  in panels of eight blocks: byte ((p * lds + r) * 8 + b) is the scale of row r's block 8 p + b, for
              ceil(k / 256) panels of lds rows (an even number of at least `rows`), on 16-byte addresses.
    Pitches of 0: dense (16 * ceil(k / 32) bytes; rows rounded up to an even number).
