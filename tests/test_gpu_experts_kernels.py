@@ -9,7 +9,7 @@ from test_gpu_experts import _sizes_of
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("rows,groups,n,k", [(2000, 3, 584, 544), (900, 5, 198, 288), (4000, 2, 4088, 800), (1500, 3, 1411, 320), (60, 6, 200, 512)])
+@pytest.mark.parametrize("rows,groups,n,k", [(2000, 3, 584, 544), (900, 5, 198, 288), (4000, 2, 4088, 800), (1500, 3, 1411, 320), (60, 6, 200, 512), (10500, 70, 520, 300)])
 def test_mxfp4_grouped_gemm_panels_of_all_groups(gpu, rows, groups, n, k):
     """Every group's matrix in the same panels, one behind the other, widths that no tile divides; the last panel ends with the last group."""
     Q, rng = gpu.MXFP4, np.random.default_rng(n)
