@@ -124,11 +124,9 @@ def work(case):
     if op == "kept":
         # forward: Z read, A and what is kept written; back: what was kept and dA read, dZ and A written
         return {"bytes": case["rows"] * case["n"] * (2 + 1 + code + code + 1 + 2 + 1), "flops": 12.0 * case["rows"] * case["n"]}
-    # a token whose target is outside the vocabulary counts nothing, and has a row of zeros in the gradient
     t, v, d, s = case["tokens"], case["vocabulary"], case["width"], _SIZE[case["type"]]
-    counted = t * (1 - case["ignored"])
-    both = s * (counted + v) * d
-    return {"bytes": both + 12.0 * t + case["grad"] * (both + s * (t + v) * d + 8.0 * t), "flops": (8.0 if case["grad"] else 2.0) * counted * v * d}
+    both = s * (t + v) * d
+    return {"bytes": both + 12.0 * t + case["grad"] * (2 * both + 8.0 * t), "flops": (8.0 if case["grad"] else 2.0) * t * v * d}
 
 
 def _assignments(gen, case):
@@ -321,11 +319,10 @@ def _plain(s):
     most = z.amax(1)
     lse = torch.log(torch.exp(z - most[:, None]).sum(1)) + most
     losses = torch.where(some, lse - z.gather(1, target[:, None])[:, 0], 0.0)
-    lse = torch.where(some, lse, 0.0)
     if not s["grad"]:
         return [losses, lse]
     share = torch.where(some, s["share"], 0.0)
-    p = torch.where(some[:, None], torch.exp(z - lse[:, None]), 0.0) * share[:, None]
+    p = torch.exp(z - lse[:, None]) * share[:, None]
     p.scatter_add_(1, target[:, None], -share[:, None])
     return [losses, lse, (p @ w).to(s["dx"].dtype), (p.t() @ x).to(s["dw"].dtype)]
 
@@ -398,11 +395,12 @@ def exact(case, seed):
     losses, lse = torch.zeros(t, dtype=torch.float64, device="cuda"), torch.zeros(t, dtype=torch.float64, device="cuda")
     dx, dw = torch.zeros_like(x), torch.zeros_like(w)
     columns = w.transpose(0, 1).contiguous()
+    for i in range(0, t, 2048):
+        lse[i:i + 2048] = torch.logsumexp(torch.matmul(x[i:i + 2048], columns), 1)
     for i in range(0, len(counted), 2048):
         these, goal = counted[i:i + 2048], target[i:i + 2048]
         z = torch.matmul(x[these], columns)
         each = torch.arange(len(these), device="cuda")
-        lse[these] = torch.logsumexp(z, 1)
         losses[these] = lse[these] - z[each, goal]
         if case["grad"]:
             p = torch.exp(z - lse[these][:, None])
