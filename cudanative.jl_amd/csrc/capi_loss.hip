@@ -33,7 +33,6 @@ namespace {
 
 using miw::loss_params;
 
-constexpr int64_t FEW_TOKENS = 64;
 using miw::LOSS_SLICED, miw::LOSS_SLICES;
 
 int check_sizes(const char *what, int64_t tokens, int64_t vocabulary, int64_t width)
@@ -56,16 +55,11 @@ struct layout {
     }
 };
 struct scores_space {
-    miw::loss_rows rows;
     float *goal_score, *stats;
 };
 scores_space take_scores(layout &l, int64_t tokens, int64_t vocabulary)
 {
     scores_space s{};
-    s.rows.place = l.take<int>(tokens);
-    s.rows.list = l.take<int>(tokens);
-    s.rows.goal = l.take<int>(tokens);
-    s.rows.offsets = l.take<int>(2);
     s.goal_score = l.take<float>(tokens);
     // (the most that any kernel makes of so many tokens or fewer: sixteen columns a slice up to 64 of them, 32 beyond)
     s.stats = l.take<float>(2 * std::max(std::min<int64_t>(tokens, 64) * (ceil_div(vocabulary, 16) + 8), tokens * (ceil_div(vocabulary, 32) + 8)));
@@ -111,14 +105,12 @@ int check_workspace(const char *what, int64_t tokens, int64_t vocabulary, int64_
     return 0;
 }
 
-// Scores: hidden rows by the vocabulary's vectors from `first` on.
-loss_params score_product(const miw::loss_rows &rows, int64_t tokens, int64_t first, int64_t columns, int64_t width, int64_t ldx, int64_t ldw, const void *X, const void *W)
+// Scores: hidden rows by the vocabulary's vectors from `first` on.  Rows are all tokens, whose targets goal has, until the caller says otherwise.
+loss_params score_product(const int *goal, int64_t tokens, int64_t first, int64_t columns, int64_t width, int64_t ldx, int64_t ldw, const void *X, const void *W)
 {
     loss_params p{};
     p.X = (const char *)W + 2 * first * ldw;
     p.Y = (const char *)X;
-    p.offsets = rows.offsets;
-    p.gather = rows.list;
     p.groups = 1;
     p.rows = p.source_rows = (int)tokens;
     p.I = (int)columns;
@@ -127,7 +119,7 @@ loss_params score_product(const miw::loss_rows &rows, int64_t tokens, int64_t fi
     p.ldy = 2 * ldx;
     p.x_k_major = 1;
     p.vector = aligned(X, 16) && aligned(W, 16) && ldx % 8 == 0 && ldw % 8 == 0 && width % 8 == 0;
-    p.goal = rows.goal;
+    p.goal = goal;
     p.first = first;
     return p;
 }
@@ -166,22 +158,14 @@ int miw_cross_entropy(int dtype, int64_t tokens, int64_t vocabulary, int64_t wid
     const int cus = miw::api_cu_count();
     layout l{(char *)workspace};
     const scores_space at = take_scores(l, tokens, vocabulary);
-    // A few tokens are not looked at first: all have a row, and the vocabulary's vectors, read once for up to 64 rows, are the time anyhow.  A row that does not
-    // count is read then; what comes of it is nobody's.
-    const bool look = tokens > FEW_TOKENS;
-    if (look) HIP_TRY(miw::launch_loss_look({at.rows, targets, nullptr, nullptr, (int)tokens, 1, 0, (long)vocabulary}, s));
-    miw::loss_rows rows = at.rows;
-    if (!look) {
-        rows.list = rows.offsets = nullptr;
-        rows.goal = const_cast<int *>(targets);
-    }
-    loss_params p = score_product(rows, tokens, 0, vocabulary, width, ldx, ldw, X, W);
+    // (every token has scores, whatever its target: lse is theirs)
+    loss_params p = score_product(targets, tokens, 0, vocabulary, width, ldx, ldw, X, W);
     const miw::loss_slices slices = miw::loss_score_slices(p, cus);
     p.stats = at.stats;
     p.goal_score = at.goal_score;
     p.stat_rows = tokens;
     HIP_TRY(miw::launch_loss_scores(p, dtype, cus, s));
-    HIP_TRY(miw::launch_loss_join({look ? at.rows.place : nullptr, targets, at.stats, at.goal_score, losses, lse, (int)tokens, slices.count, (long)tokens, (long)vocabulary}, s));
+    HIP_TRY(miw::launch_loss_join({targets, at.stats, at.goal_score, losses, lse, (int)tokens, slices.count, (long)tokens, (long)vocabulary}, s));
     return 0;
 }
 
@@ -243,7 +227,7 @@ int miw_cross_entropy_grad(int dtype, int dw_type, int accumulate, int64_t token
     sum.ldd = lddw;
     sum.accumulate = accumulate != 0;
     sum.unscale = unscale;
-    sum.vector = score_product(at.rows, tokens, 0, vocabulary, width, ldx, ldw, X, W).vector;
+    sum.vector = score_product(at.rows.goal, tokens, 0, vocabulary, width, ldx, ldw, X, W).vector;
     sum.d_vector = stores_vectors(dW, lddw, 0, type_size(dw_type), false);
     auto sum_of = [&](int64_t first, int64_t n) {
         loss_params q = sum;
@@ -261,7 +245,9 @@ int miw_cross_entropy_grad(int dtype, int dw_type, int accumulate, int64_t token
     }
     for (int64_t first = 0; first < vocabulary; first += columns) {
         const int64_t n = std::min(columns, vocabulary - first);
-        loss_params p = score_product(at.rows, tokens, first, n, width, ldx, ldw, X, W);
+        loss_params p = score_product(at.rows.goal, tokens, first, n, width, ldx, ldw, X, W);
+        p.offsets = at.rows.offsets;
+        p.gather = at.rows.list;
         p.lse = at.rows.lse;
         p.share = at.rows.share;
         p.D = at.probabilities;

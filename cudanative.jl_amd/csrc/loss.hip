@@ -9,7 +9,7 @@
 
 namespace miw {
 
-// Which tokens count, in one workgroup: a token whose target is outside the vocabulary has no row in any product.  8192 tokens at a time, every
+// Which tokens count, in one workgroup: a token whose target is outside the vocabulary has no row in any product of the gradient.  8192 tokens at a time, every
 // wavefront 64 neighbours in each of eight turns, so that all loads and nearly all stores are whole lines; the counts of the 128
 // runs of 64 are summed up in LDS, so rows keep the tokens' order.
 constexpr int LOOK_THREADS = 1024, LOOK_TURNS = 8, LOOK_WAVES = LOOK_THREADS / 64;
@@ -18,9 +18,8 @@ __global__ __launch_bounds__(LOOK_THREADS) void k_loss_look(loss_look_params p)
     __shared__ int upto[LOOK_TURNS * LOOK_WAVES];
     __shared__ unsigned largest[LOOK_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const bool grad = p.shares != nullptr;
     float scale = 1.f;
-    if (grad && p.scaled) {
+    if (p.scaled) {
         // The power of two that brings the largest finite share to 2^14 .. 2^15: shares times probabilities then use Float16's whole range.
         unsigned most = 0;
         for (int t = tid; t < p.tokens; t += LOOK_THREADS) {
@@ -47,8 +46,8 @@ __global__ __launch_bounds__(LOOK_THREADS) void k_loss_look(loss_look_params p)
         for (int e = 0; e < LOOK_TURNS; e++) {
             const int t = min(t0 + e * LOOK_THREADS + tid, p.tokens - 1);
             target[e] = p.targets[t];
-            lse[e] = grad ? p.lse[t] : 0.f;
-            share[e] = grad ? p.shares[t] : 0.f;
+            lse[e] = p.lse[t];
+            share[e] = p.shares[t];
         }
         unsigned long counted[LOOK_TURNS];
 #pragma unroll
@@ -77,10 +76,8 @@ __global__ __launch_bounds__(LOOK_THREADS) void k_loss_look(loss_look_params p)
             if (target[e] < 0) continue;
             p.rows.list[row] = t;
             p.rows.goal[row] = target[e];
-            if (grad) {
-                p.rows.lse[row] = lse[e];
-                p.rows.share[row] = share[e] * scale;
-            }
+            p.rows.lse[row] = lse[e];
+            p.rows.share[row] = share[e] * scale;
         }
         before += upto[LOOK_TURNS * LOOK_WAVES - 1];
     }
@@ -88,7 +85,7 @@ __global__ __launch_bounds__(LOOK_THREADS) void k_loss_look(loss_look_params p)
         p.rows.offsets[0] = 0;
         p.rows.offsets[1] = before;
     }
-    if (grad && p.slices > 1) {
+    if (p.slices > 1) {
         for (int g = 0; g <= p.slices; g++) {
             if (tid == 0) p.rows.slice_offsets[g] = g * before;
             if (g < p.slices)
@@ -134,18 +131,13 @@ __global__ __launch_bounds__(THREADS) void k_loss_join(loss_join_params p)
     __shared__ f32x2 parts[WAVES][COLUMNS];
     const int tid = threadIdx.x, column = tid % COLUMNS, lane = tid / COLUMNS;
     const int token = (int)blockIdx.x * COLUMNS + column;
-    int row = -1;
-    if (token < p.tokens) {
-        if (p.place) row = p.place[token];
-        else if (p.targets[token] >= 0 && p.targets[token] < p.vocabulary) row = token;
-    }
     f32x2 all = {-__builtin_inff(), 0.f};
-    if (row >= 0)
+    if (token < p.tokens)
         for (int n = lane; n < p.slices; n += 8 * LANES) {
             // eight on the way at a time
             f32x2 v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = *(const f32x2 *)(p.stats + 2 * ((long)min(n + e * LANES, p.slices - 1) * p.stat_rows + row));
+            for (int e = 0; e < 8; e++) v[e] = *(const f32x2 *)(p.stats + 2 * ((long)min(n + e * LANES, p.slices - 1) * p.stat_rows + token));
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 if (n + e * LANES < p.slices) all = joined(all, v[e]);
@@ -157,8 +149,10 @@ __global__ __launch_bounds__(THREADS) void k_loss_join(loss_join_params p)
     if (lane || token >= p.tokens) return;
     for (int n = 1; n < WAVES; n++) all = joined(all, parts[n][column]);
     const float lse = (all[0] == -__builtin_inff() ? 0.f : all[0]) + logf(all[1]);
-    p.lse[token] = row >= 0 ? lse : 0.f;
-    p.losses[token] = row >= 0 ? lse - p.goal_score[row] : 0.f;
+    const bool counts = p.targets[token] >= 0 && p.targets[token] < p.vocabulary;
+    // (a row of padding that nobody filled may hold anything: no NaN comes of it)
+    p.lse[token] = !counts && lse != lse ? 0.f : lse;
+    p.losses[token] = counts ? lse - p.goal_score[token] : 0.f;
 }
 
 hipError_t launch_loss_join(const loss_join_params &p, hipStream_t s)

@@ -4,7 +4,8 @@
 
 namespace miw {
 
-// A product whose ends the loss has of its own (loss_ends.hpp).  Rows are those tokens that count, in their order: row r is token list[r].
+// A product whose ends the loss has of its own (loss_ends.hpp).  Rows are all tokens in the scores, and those that count, in their order, in the gradient: row r is
+// token list[r].
 struct loss_params : grouped_params {
     const int *goal;        // target of each row
     float *stats;           // scores: largest score and sum of exponentials of each slice of columns and row, two values together
@@ -19,12 +20,11 @@ struct loss_params : grouped_params {
     int dense;              // gradient to the vocabulary's vectors: X's rows lie in their order
 };
 
-// What is known of the tokens once they have been looked at.  All arrays are in the workspace.
+// What the gradient knows of the tokens once they have been looked at.  All arrays are in the workspace.
 struct loss_rows {
     int *place;            // of each token: its row, or -1
     int *list, *goal;      // of each row: its token and target
     int *offsets;          // 0 and the number of rows
-    // for the gradient
     float *lse, *share;    // of each row
     float *scale;          // the power of two that shares are multiplied by, and its inverse
     int *slice_offsets, *slice_rows;  // groups of the same rows, one for each slice of a sum
@@ -32,7 +32,7 @@ struct loss_rows {
 struct loss_look_params {
     loss_rows rows;
     const int *targets;
-    const float *lse, *shares;  // shares null: no gradient
+    const float *lse, *shares;
     int tokens, slices, scaled;
     long vocabulary;
 };
@@ -50,8 +50,7 @@ hipError_t launch_loss_copy(const loss_copy_params &p, hipStream_t s);
 
 // Losses from the slices' statistics.
 struct loss_join_params {
-    const int *place;    // or null: every token has its own row
-    const int *targets;  // for that case
+    const int *targets;
     const float *stats, *goal_score;
     float *losses, *lse;
     int tokens, slices;

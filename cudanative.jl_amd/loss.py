@@ -2,7 +2,7 @@
 
 The scores are the product of X (tokens x width, what a model ends in) and W (vocabulary x width).  `cross_entropy` sums their
 exponentials up where they are made; `cross_entropy_grad` makes them again, a piece of the vocabulary at a time.  A token whose
-target is outside the vocabulary (-1, say) does not count and costs nothing.
+target is outside the vocabulary (-1, say) does not count: it has an lse, a loss of 0 and no part in the gradient.
 
 No counterpart in the reference; the products are the chain of mma calls of docs/src/device/wmma.md:51-52.  Arrays are
 DeviceArrays or raw device addresses; matrices are row-major, a pitch of 0 means dense.  All calls are asynchronous on `stream`.
@@ -22,8 +22,8 @@ def cross_entropy_workspace(tokens, vocabulary, width, *, grad=False, piece=0):
 
 
 def cross_entropy(X, W, targets, losses, lse, *, tokens, vocabulary, width, dtype=Float16, ldx=0, ldw=0, workspace, stream=None):
-    """losses[t] = lse[t] - X[t] . W[targets[t]] with lse[t] = log(sum over v of exp(X[t] . W[v])); Float32, 0 for tokens that do
-    not count.  targets: Int32.  workspace: a DeviceArray of cross_entropy_workspace bytes."""
+    """losses[t] = lse[t] - X[t] . W[targets[t]] with lse[t] = log(sum over v of exp(X[t] . W[v])); Float32.  Losses are 0 for
+    tokens that do not count, and so is their lse where their row of X makes it no number.  targets: Int32.  workspace: a DeviceArray of cross_entropy_workspace bytes."""
     call(_library.miw_cross_entropy, TYPE_CODES[dtype], tokens, vocabulary, width, ldx, ldw, X, W, targets, losses, lse, workspace,
          0 if workspace is None else workspace.nbytes, None if stream is None else _stream(stream))
 

@@ -476,8 +476,8 @@ int miw_fp8_gated_silu_grad(int dtype, int64_t rows, int64_t n, int64_t ldq, int
    each of the words), both of dtype F16 or BF16, without storing Z.  No counterpart in the reference.
      lse[t]    = log(sum over v of exp(Z[t][v]))
      losses[t] = lse[t] - Z[t][targets[t]]
-   A token whose target is outside 0 .. vocabulary - 1 does not count: its loss and lse are 0, what its row of X holds changes nothing, and the gradient has zeros
-   there and nothing of it in dW.  Scores, their exponentials' sums, losses and lse are Float32.
+   lse is every token's.  One whose target is outside 0 .. vocabulary - 1 does not count: its loss is 0, and the gradient has zeros there and nothing of it in dW; its lse
+   reaches nothing else, and is 0 where what its row of X holds makes it no number (padding that nobody filled).  Scores, their exponentials' sums, losses and lse are Float32.
      dX[t] = dlosses[t] * (sum over v of softmax(Z[t])[v] * W[v] - W[targets[t]])
      dW[v] = sum over t of dlosses[t] * (softmax(Z[t])[v] - [v = targets[t]]) * X[t]
    The gradient makes the scores again from X, W and lse, `piece` columns of the vocabulary at a time (0: the library's choice, up to 256 MiB of them or 8192 columns), and keeps

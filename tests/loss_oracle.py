@@ -17,6 +17,13 @@ def cross_entropy(x, w, targets):
     return losses, lse
 
 
+def log_sums(x, w):
+    """lse of every token, whatever its target."""
+    z = scores(x, w)
+    most = z.max(1)
+    return most + np.log(np.exp(z - most[:, None]).sum(1))
+
+
 def gradient(x, w, targets, dlosses):
     """(dX, dW, the probabilities that made them and the rows that count)."""
     some = (targets >= 0) & (targets < len(w))
