@@ -48,6 +48,11 @@ struct loss_end {
     }
 };
 
+// Which of the columns from i on a target is.  Targets are any Int32: those outside the vocabulary lie behind all columns (of at most 2^26 and a tile).
+constexpr unsigned target_column(int target, int i) { return (unsigned)target - (unsigned)i; }
+static_assert(target_column(70, 64) == 6 && target_column(63, 64) > 1u << 30 && target_column(-2147483647 - 1, (1 << 26) + 256) > 1u << 30 && target_column(-1, 0) > 1u << 30 &&
+              target_column(2147483647, (1 << 26) + 256) > 1u << 30);
+
 // Scores: of a wavefront's columns, the largest and the sum of the exponentials of the differences to it, and the target's score where it is
 // among them.  Nothing else of the scores is kept.
 struct loss_score_end : loss_end {
@@ -60,7 +65,7 @@ struct loss_score_end : loss_end {
         for (int b = 0; b < TJ; b++) {
             const int j = j0 + 16 * b + r;
             const bool here = j < t.last;
-            const int goal = here ? p.goal[j] - i : -1;
+            const unsigned goal = here ? target_column(p.goal[j], i) : ~0u;
             float most = -__builtin_inff(), score = 0.f;
 #pragma unroll
             for (int a = 0; a < TI; a++)
@@ -69,7 +74,7 @@ struct loss_score_end : loss_end {
                     const float v = i + 16 * a + e < p.I ? acc[a][b][e] : -__builtin_inff();
                     acc[a][b][e] = v;
                     most = fmaxf(most, v);
-                    score = goal == 16 * a + e ? v : score;
+                    score = goal == 16u * a + e ? v : score;
                 }
             most = across_max(most);
             // (a slice of -inf alone has no exponentials)
@@ -82,7 +87,7 @@ struct loss_score_end : loss_end {
             sum = across_sum(sum);
             if (here) {
                 if (q == 0) *(f32x2 *)(stats + 2 * (long)j) = f32x2{most, sum};
-                if (goal >= 0 && goal < 16 * TI && (goal & 15) < 4) p.goal_score[j] = score;
+                if (goal < 16 * TI && (goal & 15) < 4) p.goal_score[j] = score;
             }
         }
     }
