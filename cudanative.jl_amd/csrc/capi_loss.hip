@@ -55,12 +55,12 @@ struct layout {
     }
 };
 struct scores_space {
-    float *goal_score, *stats;
+    float *goals, *stats;
 };
 scores_space take_scores(layout &l, int64_t tokens, int64_t vocabulary)
 {
     scores_space s{};
-    s.goal_score = l.take<float>(tokens);
+    s.goals = l.take<float>(2 * tokens);
     // (the most that any kernel makes of so many tokens or fewer: sixteen columns a slice up to 64 of them, 32 beyond)
     s.stats = l.take<float>(2 * std::max(std::min<int64_t>(tokens, 64) * (ceil_div(vocabulary, 16) + 8), tokens * (ceil_div(vocabulary, 32) + 8)));
     return s;
@@ -162,10 +162,10 @@ int miw_cross_entropy(int dtype, int64_t tokens, int64_t vocabulary, int64_t wid
     loss_params p = score_product(targets, tokens, 0, vocabulary, width, ldx, ldw, X, W);
     const miw::loss_slices slices = miw::loss_score_slices(p, cus);
     p.stats = at.stats;
-    p.goal_score = at.goal_score;
+    p.goals = at.goals;
     p.stat_rows = tokens;
     HIP_TRY(miw::launch_loss_scores(p, dtype, cus, s));
-    HIP_TRY(miw::launch_loss_join({targets, at.stats, at.goal_score, losses, lse, (int)tokens, slices.count, (long)tokens, (long)vocabulary}, s));
+    HIP_TRY(miw::launch_loss_join({targets, at.stats, at.goals, losses, lse, (int)tokens, slices.count, slices.width, (long)tokens, (long)vocabulary}, s));
     return 0;
 }
 

@@ -116,11 +116,15 @@ hipError_t launch_loss_copy(const loss_copy_params &p, hipStream_t s)
     return hipGetLastError();
 }
 
-// Two sums of exponentials, each over the largest of its scores, as one.
-__device__ inline f32x2 joined(f32x2 a, f32x2 b)
+// Sums of exponentials, over the largest of their scores: of all words, and of those that are not the target.
+struct loss_sum {
+    float most, all, others;
+};
+// Two of them as one.
+__device__ inline loss_sum joined(const loss_sum &a, const loss_sum &b)
 {
-    const float most = fmaxf(a[0], b[0]), from = most == -__builtin_inff() ? 0.f : most;
-    return f32x2{most, a[1] * exp_of(a[0] - from) + b[1] * exp_of(b[0] - from)};
+    const float most = fmaxf(a.most, b.most), from = most == -__builtin_inff() ? 0.f : most, fa = exp_of(a.most - from), fb = exp_of(b.most - from);
+    return {most, a.all * fa + b.all * fb, a.others * fa + b.others * fb};
 }
 // COLUMNS tokens a workgroup, THREADS / COLUMNS lanes each over the slices; those of a wavefront meet by exchanges, the wavefronts in LDS in their order.
 // (Four tokens a workgroup where they are few: 16 tokens, 2048 slices 9.9 us with sixteen.)
@@ -128,11 +132,15 @@ template <int THREADS, int COLUMNS>
 __global__ __launch_bounds__(THREADS) void k_loss_join(loss_join_params p)
 {
     constexpr int LANES = THREADS / COLUMNS, WAVES = THREADS / 64;
-    __shared__ f32x2 parts[WAVES][COLUMNS];
+    __shared__ loss_sum parts[WAVES][COLUMNS];
     const int tid = threadIdx.x, column = tid % COLUMNS, lane = tid / COLUMNS;
     const int token = (int)blockIdx.x * COLUMNS + column;
-    f32x2 all = {-__builtin_inff(), 0.f};
-    if (token < p.tokens)
+    const int target = token < p.tokens ? p.targets[token] : -1;
+    const bool counts = target >= 0 && target < p.vocabulary;
+    const f32x2 goal = counts ? *(const f32x2 *)(p.goals + 2l * token) : f32x2{0.f, 0.f};
+    loss_sum sum = {-__builtin_inff(), 0.f, 0.f};
+    if (token < p.tokens) {
+        const int goal_slice = counts ? target / p.slice : -1;
         for (int n = lane; n < p.slices; n += 8 * LANES) {
             // eight on the way at a time
             f32x2 v[8];
@@ -140,19 +148,21 @@ __global__ __launch_bounds__(THREADS) void k_loss_join(loss_join_params p)
             for (int e = 0; e < 8; e++) v[e] = *(const f32x2 *)(p.stats + 2 * ((long)min(n + e * LANES, p.slices - 1) * p.stat_rows + token));
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (n + e * LANES < p.slices) all = joined(all, v[e]);
+                if (n + e * LANES < p.slices) sum = joined(sum, {v[e][0], v[e][1], n + e * LANES == goal_slice ? goal[1] : v[e][1]});
         }
+    }
 #pragma unroll
-    for (int step = COLUMNS; step < 64; step *= 2) all = joined(all, f32x2{__shfl_xor(all[0], step), __shfl_xor(all[1], step)});
-    if ((tid & 63) < COLUMNS) parts[tid >> 6][column] = all;
+    for (int step = COLUMNS; step < 64; step *= 2) sum = joined(sum, {__shfl_xor(sum.most, step), __shfl_xor(sum.all, step), __shfl_xor(sum.others, step)});
+    if ((tid & 63) < COLUMNS) parts[tid >> 6][column] = sum;
     __syncthreads();
     if (lane || token >= p.tokens) return;
-    for (int n = 1; n < WAVES; n++) all = joined(all, parts[n][column]);
-    const float lse = (all[0] == -__builtin_inff() ? 0.f : all[0]) + logf(all[1]);
-    const bool counts = p.targets[token] >= 0 && p.targets[token] < p.vocabulary;
+    for (int n = 1; n < WAVES; n++) sum = joined(sum, parts[n][column]);
+    const float lse = (sum.most == -__builtin_inff() ? 0.f : sum.most) + logf(sum.all);
     // (a row of padding that nobody filled may hold anything: no NaN comes of it)
     p.lse[token] = !counts && lse != lse ? 0.f : lse;
-    p.losses[token] = counts ? lse - p.goal_score[token] : 0.f;
+    // Where the target's score is the largest the loss is log1p of the others' sum, which keeps the digits of a loss far below 1.
+    const float over = sum.most - goal[0];
+    p.losses[token] = !counts ? 0.f : over == 0.f ? log1pf(sum.others) : over + logf(sum.all);
 }
 
 hipError_t launch_loss_join(const loss_join_params &p, hipStream_t s)

@@ -9,7 +9,7 @@ namespace miw {
 struct loss_params : grouped_params {
     const int *goal;        // target of each row
     float *stats;           // scores: largest score and sum of exponentials of each slice of columns and row, two values together
-    float *goal_score;      // scores: of each row
+    float *goals;           // scores: of each row the target's, and its slice's sum without it
     long stat_rows;         // rows that a slice of stats has room for
     const float *lse;       // probabilities: of each row
     const float *share;     // probabilities: of each row, times the power of two that keeps Float16 in range
@@ -51,9 +51,9 @@ hipError_t launch_loss_copy(const loss_copy_params &p, hipStream_t s);
 // Losses from the slices' statistics.
 struct loss_join_params {
     const int *targets;
-    const float *stats, *goal_score;
+    const float *stats, *goals;
     float *losses, *lse;
-    int tokens, slices;
+    int tokens, slices, slice;  // columns of a slice
     long stat_rows, vocabulary;
 };
 hipError_t launch_loss_join(const loss_join_params &p, hipStream_t s);

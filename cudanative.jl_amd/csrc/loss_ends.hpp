@@ -53,8 +53,9 @@ constexpr unsigned target_column(int target, int i) { return (unsigned)target - 
 static_assert(target_column(70, 64) == 6 && target_column(63, 64) > 1u << 30 && target_column(-2147483647 - 1, (1 << 26) + 256) > 1u << 30 && target_column(-1, 0) > 1u << 30 &&
               target_column(2147483647, (1 << 26) + 256) > 1u << 30);
 
-// Scores: of a wavefront's columns, the largest and the sum of the exponentials of the differences to it, and the target's score where it is
-// among them.  Nothing else of the scores is kept.
+// Scores: of a wavefront's columns, the largest and the sum of the exponentials of the differences to it; and of the target, where it is among them, its score and that sum
+// without it.  Nothing else of the scores is kept.  (The loss is log(1 + the others' exponentials over the target's); in a sum that has the target's too, 1 where its score is the
+// largest, what is far below 1 is lost.)
 struct loss_score_end : loss_end {
     template <class DT, class PARAMS, int TI, int TJ>
     static __device__ __forceinline__ void finish(const PARAMS &p, const grouped_tile &t, f32x4 (&acc)[TI][TJ], int i0, int j0, int lane)
@@ -66,7 +67,7 @@ struct loss_score_end : loss_end {
             const int j = j0 + 16 * b + r;
             const bool here = j < t.last;
             const unsigned goal = here ? target_column(p.goal[j], i) : ~0u;
-            float most = -__builtin_inff(), score = 0.f;
+            float most = -__builtin_inff();
 #pragma unroll
             for (int a = 0; a < TI; a++)
 #pragma unroll
@@ -74,7 +75,6 @@ struct loss_score_end : loss_end {
                     const float v = i + 16 * a + e < p.I ? acc[a][b][e] : -__builtin_inff();
                     acc[a][b][e] = v;
                     most = fmaxf(most, v);
-                    score = goal == 16u * a + e ? v : score;
                 }
             most = across_max(most);
             // (a slice of -inf alone has no exponentials)
@@ -85,10 +85,20 @@ struct loss_score_end : loss_end {
 #pragma unroll
                 for (int e = 0; e < 4; e++) sum += exp_of(acc[a][b][e] - from);
             sum = across_sum(sum);
-            if (here) {
-                if (q == 0) *(f32x2 *)(stats + 2 * (long)j) = f32x2{most, sum};
-                if (goal < 16 * TI && (goal & 15) < 4) p.goal_score[j] = score;
-            }
+            if (here && q == 0) *(f32x2 *)(stats + 2 * (long)j) = f32x2{most, sum};
+            const bool mine = goal < 16 * TI && (goal & 15) < 4;
+            if (!__any(mine)) continue;  // (few wavefronts have a target of their rows among their columns)
+            float score = 0.f, others = 0.f;
+#pragma unroll
+            for (int a = 0; a < TI; a++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool target = goal == 16u * a + e;
+                    score = target ? acc[a][b][e] : score;
+                    others += target ? 0.f : exp_of(acc[a][b][e] - from);
+                }
+            others = across_sum(others);
+            if (mine) *(f32x2 *)(p.goals + 2 * (long)j) = f32x2{score, others};
         }
     }
 };

@@ -475,7 +475,7 @@ int miw_fp8_gated_silu_grad(int dtype, int64_t rows, int64_t n, int64_t ldq, int
 /* Softmax cross entropy of tokens x vocabulary scores Z = X * W^T, X tokens x width (what a model ends in) and W vocabulary x width (a vector for
    each of the words), both of dtype F16 or BF16, without storing Z.  No counterpart in the reference.
      lse[t]    = log(sum over v of exp(Z[t][v]))
-     losses[t] = lse[t] - Z[t][targets[t]]
+     losses[t] = lse[t] - Z[t][targets[t]]   (summed up so that a loss far below 1 keeps its digits)
    lse is every token's.  One whose target is outside 0 .. vocabulary - 1 does not count: its loss is 0, and the gradient has zeros there and nothing of it in dW; its lse
    reaches nothing else, and is 0 where what its row of X holds makes it no number (padding that nobody filled).  Scores, their exponentials' sums, losses and lse are Float32.
      dX[t] = dlosses[t] * (sum over v of softmax(Z[t])[v] * W[v] - W[targets[t]])
