@@ -61,8 +61,7 @@ scores_space take_scores(layout &l, int64_t tokens, int64_t vocabulary)
 {
     scores_space s{};
     s.goals = l.take<float>(2 * tokens);
-    // (the most that any kernel makes of so many tokens or fewer: sixteen columns a slice up to 64 of them, 32 beyond)
-    s.stats = l.take<float>(2 * std::max(std::min<int64_t>(tokens, 64) * (ceil_div(vocabulary, 16) + 8), tokens * (ceil_div(vocabulary, 32) + 8)));
+    s.stats = l.take<float>(2 * miw::loss_stats(tokens, vocabulary));
     return s;
 }
 struct gradient_space {
@@ -158,14 +157,19 @@ int miw_cross_entropy(int dtype, int64_t tokens, int64_t vocabulary, int64_t wid
     const int cus = miw::api_cu_count();
     layout l{(char *)workspace};
     const scores_space at = take_scores(l, tokens, vocabulary);
-    // (every token has scores, whatever its target: lse is theirs)
-    loss_params p = score_product(targets, tokens, 0, vocabulary, width, ldx, ldw, X, W);
-    const miw::loss_slices slices = miw::loss_score_slices(p, cus);
-    p.stats = at.stats;
-    p.goals = at.goals;
-    p.stat_rows = tokens;
-    HIP_TRY(miw::launch_loss_scores(p, dtype, cus, s));
-    HIP_TRY(miw::launch_loss_join({targets, at.stats, at.goals, losses, lse, (int)tokens, slices.count, slices.width, (long)tokens, (long)vocabulary}, s));
+    // Every token has scores, whatever its target: lse is theirs.  All in one go, unless their statistics have no room; then the last run has tokens of the one before
+    // again, since its kernel, and so its slices, go by the number of tokens.
+    const int64_t run = miw::loss_run(score_product(targets, tokens, 0, vocabulary, width, ldx, ldw, X, W), cus);
+    for (int64_t done = 0; done < tokens; done += run) {
+        const int64_t first = std::min(done, tokens - run);
+        loss_params p = score_product(targets + first, run, 0, vocabulary, width, ldx, ldw, (const char *)X + 2 * first * ldx, W);
+        const miw::loss_slices slices = miw::loss_score_slices(p, cus);
+        p.stats = at.stats;
+        p.goals = at.goals;
+        p.stat_rows = run;
+        HIP_TRY(miw::launch_loss_scores(p, dtype, cus, s));
+        HIP_TRY(miw::launch_loss_join({targets + first, at.stats, at.goals, losses + first, lse + first, (int)run, slices.count, slices.width, (long)run, (long)vocabulary}, s));
+    }
     return 0;
 }
 

@@ -84,6 +84,10 @@ struct loss_cut {
 loss_cut cut_loss_rows(long tokens, long width, long columns, int cus);
 grouped_choice choose_loss_rows(const grouped_params &p, int cus);
 loss_slices loss_score_slices(const grouped_params &p, int cus);
+// Statistics (slices times tokens) that the workspace has room for, and the tokens that scores are made of at a time, all in that room, of p.rows.
+constexpr int64_t LOSS_STATS = 1 << 24, LOSS_RUN = 256;
+long loss_stats(long tokens, long vocabulary);
+long loss_run(grouped_params p, int cus);
 bool loss_sum_is_dense(const grouped_params &p, int cus);  // the vectors' gradient, of the first and longest piece
 hipError_t launch_loss_scores(const loss_params &p, int dtype, int cus, hipStream_t s);
 hipError_t launch_loss_probabilities(const loss_params &p, int dtype, int cus, hipStream_t s);

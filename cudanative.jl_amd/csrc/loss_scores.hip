@@ -6,6 +6,8 @@
 
 namespace miw {
 
+static long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
 // As grouped products are, but for a few rows: the vocabulary is one group of many columns, read once, and what counts is how much of it is on the way
 // (bf16, weights of repeated calls; microseconds with the join).
 //   Up to sixteen rows go straight into registers: from HBM, 16 rows, 32768 x 4096 57 on four wavefronts a workgroup, 62 on 128 x 64 tiles.  Two wavefronts where
@@ -38,6 +40,26 @@ loss_slices loss_score_slices(const grouped_params &p, int cus)
     case TILE_256x256: return slices(256, 2);
     case TILE_256x128: return slices(256, 4);
     default: return slices(128, 4);
+    }
+}
+
+// 2^24 of them, 128 MiB, or those of 256 tokens where that is more.  A tile of 256 x 256 makes slices of 128 columns, so 16384 tokens by 128256 words are one run, and more
+// runs cost nothing that can be seen (x 1024 bf16: 3.36 ms, 65536 tokens in four runs 13.1; 20000 in two of 10240 4.10).
+static long all_stats(long tokens, long vocabulary)
+{
+    // (the most that any kernel makes of so many tokens or fewer: sixteen columns a slice up to 64 of them, 32 beyond)
+    return std::max(std::min(tokens, 64l) * (ceil_div(vocabulary, 16) + 8), tokens * (ceil_div(vocabulary, 32) + 8));
+}
+long loss_stats(long tokens, long vocabulary) { return std::min(all_stats(tokens, vocabulary), std::max((long)LOSS_STATS, all_stats(LOSS_RUN, vocabulary))); }
+long loss_run(grouped_params p, int cus)
+{
+    const long tokens = p.rows, room = loss_stats(tokens, p.I);
+    for (long runs = 1;;) {
+        const long run = runs == 1 ? tokens : std::min(tokens, ceil_div(ceil_div(tokens, runs), LOSS_RUN) * LOSS_RUN);
+        p.rows = p.source_rows = (int)run;
+        const long need = run * loss_score_slices(p, cus).count;
+        if (need <= room) return run;
+        runs = std::max(runs + 1, runs * need / room);
     }
 }
 

@@ -41,3 +41,14 @@ def loss_kernels(miw, tokens, vocabulary, width, cus=256):
     names += ["%d x %s" % (cut.slices, "plain" if plain else TILES[cut.tile])]
     p = _GroupedParams(groups=1, rows=tokens, source_rows=tokens, I=width, J=vocabulary + 7 & -8, ldx=2 * width, ldy=2 * columns, vector=vector)
     return names + ["dense" if sum_is_dense(miw, p, cus) else _name(grouped(ctypes.byref(p), False, True, cus))]
+
+
+def score_run(miw, tokens, vocabulary, width, vector=True, cus=256):
+    """Tokens that scores are made of at a time, and the slices of the vocabulary that each of them has statistics of."""
+    class Slices(ctypes.Structure):
+        _fields_ = [("width", ctypes.c_int), ("count", ctypes.c_int)]
+
+    p = _GroupedParams(groups=1, rows=tokens, source_rows=tokens, I=vocabulary, K=width, ldx=2 * width, ldy=2 * width, x_k_major=1, vector=vector)
+    run = _rule(miw, "_ZN3miw8loss_runENS_14grouped_paramsEi", ctypes.c_long, _GroupedParams, ctypes.c_int)(p, cus)
+    p.rows = p.source_rows = run
+    return run, _rule(miw, "_ZN3miw17loss_score_slicesERKNS_14grouped_paramsEi", Slices, ctypes.POINTER(_GroupedParams), ctypes.c_int)(ctypes.byref(p), cus).count
