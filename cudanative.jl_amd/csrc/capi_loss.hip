@@ -90,11 +90,11 @@ gradient_space take_gradient(layout &l, int64_t tokens, int64_t vocabulary, int6
 
 size_t workspace_bytes_of(int64_t tokens, int64_t vocabulary, int64_t width, bool grad, int64_t piece)
 {
-    layout l{nullptr};
     if (tokens == 0) return 0;
-    if (grad) take_gradient(l, tokens, vocabulary, width, piece);
-    else take_scores(l, tokens, vocabulary);
-    return l.used;
+    layout scores{nullptr}, gradient{nullptr};
+    take_scores(scores, tokens, vocabulary);
+    if (grad) take_gradient(gradient, tokens, vocabulary, width, piece);
+    return std::max(scores.used, gradient.used);  // (a gradient's workspace does for the scores before it)
 }
 int check_workspace(const char *what, int64_t tokens, int64_t vocabulary, int64_t width, bool grad, int64_t piece, const void *workspace, size_t bytes)
 {

@@ -191,7 +191,7 @@ class Vocabulary:
     def __init__(self, pkg, W, *, tokens, vocabulary, width):
         self.pkg, self.W, self.sizes, new = pkg, W, dict(vocabulary=vocabulary, width=width), pkg.DeviceArray.undef
         self.losses, self.lse, self.dX, self.dW = new(np.float32, tokens), new(np.float32, tokens), new(np.float16, tokens * width), new(np.float32, vocabulary * width)
-        self.workspace = new(np.uint8, max(16, *(pkg.LOSS.cross_entropy_workspace(tokens, vocabulary, width, grad=grad) for grad in (False, True))))
+        self.workspace = new(np.uint8, max(16, pkg.LOSS.cross_entropy_workspace(tokens, vocabulary, width, grad=True)))
 
     def forward(self, X, targets, *, tokens, stream=None):
         """Losses of the tokens (Float32); targets outside the vocabulary do not count."""

@@ -1026,7 +1026,7 @@ end
 
 # ---------------------------------------------------------------------------- the loss ----
 
-"Bytes of workspace that cross_entropy! needs, or, with `grad`, cross_entropy_grad!."
+"Bytes of workspace that cross_entropy! needs, or, with `grad`, both it and cross_entropy_grad!."
 function cross_entropy_workspace(tokens::Integer, vocabulary::Integer, width::Integer; grad::Bool=false, piece::Integer=0)
     n = Ref{Csize_t}(0)
     check(ccall((:miw_cross_entropy_workspace, libmiwmma), Cint, (Int64, Int64, Int64, Cint, Int64, Ptr{Csize_t}), tokens, vocabulary, width,

@@ -15,7 +15,7 @@ from .wmma import Float16
 
 
 def cross_entropy_workspace(tokens, vocabulary, width, *, grad=False, piece=0):
-    """Bytes of workspace that cross_entropy needs for these sizes, or, with grad, cross_entropy_grad."""
+    """Bytes of workspace that cross_entropy needs for these sizes, or, with grad, both it and cross_entropy_grad."""
     n = ctypes.c_size_t()
     call(_library.miw_cross_entropy_workspace, tokens, vocabulary, width, 1 if grad else 0, piece, ctypes.byref(n))
     return n.value

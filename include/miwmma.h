@@ -485,8 +485,8 @@ int miw_fp8_gated_silu_grad(int dtype, int64_t rows, int64_t n, int64_t ldq, int
    largest |dlosses| lies between 2^14 and 2^15, so that only products below 2^-28 of it lose bits.  The products' sums are Float32, dX's over all pieces; they
    are rounded once.  dX (tokens x width, dtype) or dW (vocabulary x width, dtype or F32) may be null: it is not computed.  accumulate: added to what
    dW holds.  Results share no memory with operands.
-   The workspace (miw_cross_entropy_workspace bytes, 16-byte aligned, no clearing needed) is written by a call and holds nothing for the next; one for some number of
-   tokens suffices for fewer of the same vocabulary, width and piece.  Calls that overlap need one each.  At most 2^26 tokens.  Any sizes and pitches; 16-byte aligned
+   The workspace (miw_cross_entropy_workspace bytes, 16-byte aligned, no clearing needed) is written by a call and holds nothing for the next; one for the gradient
+   suffices for the scores too, and one for some number of tokens for fewer of the same vocabulary, width and piece.  Calls that overlap need one each.  At most 2^26 tokens.  Any sizes and pitches; 16-byte aligned
    operands with width and pitches in multiples of 8 elements run on the faster kernels.  The same bits every time. */
 int miw_cross_entropy_workspace(int64_t tokens, int64_t vocabulary, int64_t width, int grad, int64_t piece, size_t *bytes);
 int miw_cross_entropy(int dtype, int64_t tokens, int64_t vocabulary, int64_t width, int64_t ldx, int64_t ldw, const void *X, const void *W, const int *targets,

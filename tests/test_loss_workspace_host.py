@@ -24,3 +24,10 @@ def test_each_run_has_room(miw, vocabulary, width, vector):
         # tokens in one run where there is room for it
         assert run == tokens or 8 * tokens * slices > 1 << 27 or run * 2 > tokens, (tokens, run, slices)
     assert score_run(miw, 16384, 128256, 2048)[0] == 16384
+
+
+@pytest.mark.parametrize("vocabulary,width", [(1, 1), (5000, 64), (32003, 2048), (128256, 8), (128256, 2048), (1 << 21, 64)])
+@pytest.mark.parametrize("piece", [0, 1, 1000])
+def test_a_gradients_workspace_does_for_the_scores(miw, vocabulary, width, piece):
+    for tokens in TOKENS:
+        assert miw.LOSS.cross_entropy_workspace(tokens, vocabulary, width, grad=True, piece=piece) >= miw.LOSS.cross_entropy_workspace(tokens, vocabulary, width), tokens
