@@ -52,3 +52,21 @@ def score_run(miw, tokens, vocabulary, width, vector=True, cus=256):
     run = _rule(miw, "_ZN3miw8loss_runENS_14grouped_paramsEi", ctypes.c_long, _GroupedParams, ctypes.c_int)(p, cus)
     p.rows = p.source_rows = run
     return run, _rule(miw, "_ZN3miw17loss_score_slicesERKNS_14grouped_paramsEi", Slices, ctypes.POINTER(_GroupedParams), ctypes.c_int)(ctypes.byref(p), cus).count
+
+
+def piece_kernels(miw, tokens, vocabulary, width, asked=0, cus=256):
+    """For each piece of the vocabulary, its columns and the kernels of its probabilities, rows' gradients (with the slices) and vectors' gradients, of dense, aligned operands."""
+    scores = _rule(miw, "_ZN3miw16choose_loss_rowsERKNS_14grouped_paramsEi", _Choice, ctypes.POINTER(_GroupedParams), ctypes.c_int)
+    grouped = _rule(miw, "_ZN3miw14choose_groupedERKNS_14grouped_paramsEbbi", _Choice, ctypes.POINTER(_GroupedParams), ctypes.c_bool, ctypes.c_bool, ctypes.c_int)
+    columns = piece(miw, tokens, vocabulary, asked)
+    longest = min(columns, vocabulary)
+    cut = _rule(miw, "_ZN3miw13cut_loss_rowsEllli", _Cut, ctypes.c_long, ctypes.c_long, ctypes.c_long, ctypes.c_int)(tokens, width, longest, cus)
+
+    def sums(n):
+        return _GroupedParams(groups=1, rows=tokens, source_rows=tokens, I=width, J=n + 7 & -8, ldx=2 * width, ldy=2 * columns, vector=1)
+
+    dense, out = sum_is_dense(miw, sums(longest), cus), []  # (of the first piece, and so of all)
+    for n in [min(columns, vocabulary - first) for first in range(0, vocabulary, columns)]:
+        p = _GroupedParams(groups=1, rows=tokens, source_rows=tokens, I=n, K=width, ldx=2 * width, ldy=2 * width, x_k_major=1, vector=1)
+        out.append((n, _name(scores(ctypes.byref(p), cus)), "%d x %s" % (cut.slices, TILES[cut.tile]), "dense" if dense else _name(grouped(ctypes.byref(sums(n)), False, True, cus))))
+    return out
