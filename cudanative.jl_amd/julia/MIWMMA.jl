@@ -980,7 +980,7 @@ function fp8_dequantize!(X, codes, scales; rows::Integer, k::Integer, dtype::Sym
     return X
 end
 
-"D (m x n) = A * B^T with A in `a_format` and B in e4m3."
+"D (m x n) = A * B^T with A in `a_format` and B in e4m3; `d_type` :f32 sums up all bits of the products, results of 16 bits those above 2^-13 of the largest of eight."
 function fp8_gemm!(D, A, A_scales, B, B_scales; m::Integer, n::Integer, k::Integer, d_type::Symbol=:f16, a_format::Symbol=:e4m3,
                    epilogue::Symbol=:none, lda::Integer=0, lds_a::Integer=0, ldb::Integer=0, lds_b::Integer=0, ldd::Integer=0, stream=C_NULL)
     GC.@preserve D A A_scales B B_scales check(ccall((:miw_fp8_gemm, libmiwmma), Cint,
