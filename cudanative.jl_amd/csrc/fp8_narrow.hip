@@ -4,6 +4,7 @@
 // 128-byte blocks of k in turn, a lane loads its 32 bytes of a weight row straight into an MFMA fragment, DEPTH blocks ahead, and the partial
 // sums are added in wavefront order through LDS: no second kernel, the same bits every time.  A block's scale comes with the row's four of its panel.
 // Bound by HBM: 128 rows over 56 of 64 groups, 2048 x 2048, 235 MB in 36 to 41 us (5.7 to 6.4 TB/s, partly from the last-level cache); one group of 16 rows, 32768 x 8192, 54 to 56 us for 270 MB.
+// Float32 results, by way of bfloat16, are nearly as fast: the 64 groups 39.7 us (38.8 with 16-bit ones), 16 rows, 8192 x 8192 16.8 (15.8), 64 rows 42 (35.5).
 #include "fp8_common.hpp"
 
 namespace miw {

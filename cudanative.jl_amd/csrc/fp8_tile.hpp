@@ -7,8 +7,9 @@
 //   16-bit results: one MFMA of 128 k takes both 16-byte pieces that a lane has of a row's slot, and applies the scales.
 //   Float32 results: the pieces become bfloat16 with their scale, eight values at a time (fp8_common.hpp says why).
 //
-// Bound by the LDS reads beside the MFMAs where tiles are many (256 x 256, half a wavefront's rows at a time: 4096 x 4096 x 4096 57 us, 2.4 PFLOP/s, of x 8192 102 to 104: 83 with
-// zeros for data, 70 without loads, 72 without MFMAs), by latency where they are few (509 x 656 x 720, 48 tiles of 128 x 64 and Float32 results: 8 us). Float32
+// Bound by the power cap where tiles are many (256 x 256, half a wavefront's rows at a time: 4096 x 4096 x 4096 57 us, 2.4 PFLOP/s, x 8192 102 to 104; the latter with zeros for data 83,
+// of which the MFMAs beside LDS reads alone take 70 and the loads alone 72), by latency where they are few: 509 x 656 x 720 with Float32 results is 48 tiles of 128 x 64 on 256 CUs, each a
+// chain of six slots that are widened: 8 us, where a launch takes 3.5 (smaller tiles, or wavefronts that share k, are not there). Float32
 // results on 256 x 128: 4096 x 4096 x 8192 218 us, 1.26 PFLOP/s, nine tenths of what the 16-bit instructions reach in products of 16 bits.
 #pragma once
 #include "fp8_common.hpp"

@@ -1,7 +1,7 @@
-// Softmax cross entropy over a large vocabulary: the tokens that count, the join of the slices' statistics, and that of the rows' gradients.
+// Softmax cross entropy over a large vocabulary: the join of the scores' statistics; for the gradient the tokens that count, and the join of the rows' gradients.
 // The products are in loss_products.hpp.
 //
-// All of it is small beside them: the look 2.6 to 5 us up to 8192 tokens, one workgroup's chain of loads and barriers; the join 4.2 to 8.3 (2048 slices of 16 tokens 5.4; 252 of 8192, 16 MB, 7.8);
+// All of it is small beside them: the look 3.9 to 5 us for 509 to 4096 tokens, one workgroup's chain of loads and barriers; the join 4.2 to 7 (2048 slices of 16 tokens 5.5; 252 of 8192, 16 MB, 6.4 to 7);
 // the rows' gradients 3.8 (356 rows x 720, five slices) to 38 (8192 x 4096, 200 MB, 5.3 TB/s); the copy 12 (4096 x 4096, 64 MB) and 21 (8192 x 4096).
 #include "loss_ends.hpp"
 

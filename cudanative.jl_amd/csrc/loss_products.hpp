@@ -1,7 +1,7 @@
 // The products of the loss for one element type: the grouped kernels with the loss's ends, chosen as grouped products are.
 //
 // Scores z = x . w of all rows by the vocabulary's vectors; again, of those that count, for the probabilities, share (exp(z - lse) - [target]); and these by the vectors (the rows' gradients) and
-// by the rows (the vectors').  Bound by the matrix cores under the power cap where there is work: 4096 rows, 32768 x 4096 bf16: 750, 820, 700 and 780 us, 1.27 to 1.49
+// by the rows (the vectors').  Bound by the matrix cores under the power cap where there is work: 4096 rows, 32768 x 4096 bf16: 750, 810 to 820, 700 to 715 and 780 us, 1.27 to 1.49
 // PFLOP/s, the probabilities the slowest with their exponentials and 268 MB of stores.  Few rows: by HBM (16 rows: 48 to 52 us for 268 MB).  Few hundred rows: by latency, 11
 // to 16 us each (356 rows, 4999 x 720).
 #pragma once
